@@ -169,9 +169,8 @@ NRSE_DEV float gelu_grad_fast(float x) {
   const float cdf = x >= 0.f ? 1.0f - h : h;
   return fmaf(x * 0.39894228040143268f, e, cdf);
 }
-// Two-lane (packed FP32) forms of the same evaluation, op for op: the polynomial FMAs and
-// products issue as v_pk_fma_f32 / v_pk_mul_f32 (two elements per VALU instruction); the clamp
-// (v_med3), rcp and exp stay per element. Used where measured faster (conv0 forward, 5%; the
+// Two-lane forms of the same evaluation, op for op: packed f32 instructions in the files that the
+// Makefile lists in PACKED_F32, one instruction per lane elsewhere. Used where measured faster (conv0 forward, 5%; the
 // 256x256 GEMM's register epilogue, FFN-up +1.4 % isolated in r03 -- an r02 GEMM epilogue had
 // measured 1 % slower with it); in the LN kernels and conv0 backward the packed form was neutral
 // or slower.
