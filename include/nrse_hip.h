@@ -345,6 +345,77 @@ int nrse_attn_dropout_mask(uint16_t* drop_mask, int batch, int T, int H, float d
                            void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention over packed sequences (added to ABI 11; nothing before it changed). Sequence s is the
+ * rows [cu_seqlens[s], cu_seqlens[s + 1]) of every operand, or the first seq_lens[s] of them (a padded
+ * batch); rows of no sequence are neither read into a result nor written. hq query heads over hkv
+ * key heads (hq a multiple of hkv), head_dim 64 or 128, bf16 or f32 (exact f32 products), full or
+ * causal (key <= query). Element (row, head, d) of x is at x + row * x_row + head * x_head + d:
+ * strides in elements, 16-byte multiples, row stride >= head_dim.
+ *   s_ij = scale q_i.k_j + gate[h, i] * bias_vec[h, j - i + bias_len - 1]
+ * bias_vec [hq, 2 * bias_len - 1] f32 (NULL: none) with bias_len >= every sequence's length; gate
+ * [hq, rows] f32 (NULL: 1). A bias of -inf masks (with gate > 0); a row that is left nothing gives
+ * zeros, lse = -inf and zero gradients. lse [hq, rows] f32 natural log (the forward may pass NULL).
+ * cu_seqlens and seq_lens are device memory: what they hold is clamped to [0, rows], never trusted with
+ * an address. A key row that holds NaN or infinity can reach the rows of its own sequence within
+ * 128 rows before it under the causal mask (0 * NaN in a masked product), never another sequence.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+  uint32_t struct_size;
+  int dtype;
+  const void* q; const void* k; const void* v; void* out;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  float* lse;
+  const int* cu_seqlens;          /* [nseq + 1] */
+  const int* seq_lens;            /* [nseq] or NULL */
+  int nseq;
+  int causal;
+  long long rows;
+  int hq, hkv, head_dim;
+  float scale;
+  const float* bias_vec; const float* gate;
+  int bias_len;
+} nrse_attn_packed_fwd_params;
+
+/* dq, dk, dv are overwritten (dk, dv: summed over the query heads that share a key head, in one
+ * order). delta [hq, rows]: scratch. dgate [hq, rows] (optional, with a gate). dbias_vec (optional, with
+ * a bias): d(loss)/d(bias_vec), overwritten, or added to if accumulate; needs part, a workspace of
+ * nrse_attn_packed_bwd_workspace(p) floats. No atomics: the same inputs give the same bits. */
+typedef struct {
+  uint32_t struct_size;
+  int dtype;
+  const void* q; const void* k; const void* v; const void* out; const void* dout;
+  void* dq; void* dk; void* dv;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, dout_row, dout_head;
+  long long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  const float* lse; float* delta;
+  const int* cu_seqlens;
+  const int* seq_lens;
+  int nseq;
+  int causal;
+  long long rows;
+  int hq, hkv, head_dim;
+  float scale;
+  const float* bias_vec; const float* gate;
+  int bias_len;
+  int accumulate;
+  float* dgate; float* dbias_vec;
+  float* part;
+} nrse_attn_packed_bwd_params;
+
+int nrse_attn_packed_fwd(const nrse_attn_packed_fwd_params* p, void* stream);
+int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* stream);
+long long nrse_attn_packed_bwd_workspace(const nrse_attn_packed_bwd_params* p);
+
+/* The bias vector of a learned table by buckets, for any length without a table per length: edges [n]
+ * int32 ascending from 0 are the smallest distances of the n buckets of one side
+ * (nrse_amd.hostside.bucket_edges). Two-sided (causal = 0): E [2n, H], keys at or behind the query take
+ * rows 0 .. n-1, keys ahead n .. 2n-1. causal = 1: E [n, H], and a key ahead counts as distance 0.
+ *   vec[h, d + T - 1] = E[bucket(d), h], |d| < T;   dE[b, h] (+)= sum of dvec[h, d + T - 1] over bucket b */
+int nrse_rel_bias_expand(const float* E, const int* edges, int n, float* vec, int H, int T, int causal, void* stream);
+int nrse_rel_bias_collect(const float* dvec, const int* edges, int n, float* dE, int H, int T, int causal,
+                          int accumulate, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Conv feature encoder front end and the positional-conv weight norm.
  * conv0 = Conv1d(1 -> C, k, stride s, no bias) + LN(C) + GELU ([TF]modeling_wavlm.py:712-720),
  * channels-last output [B, T0, C]. Backward recomputes conv0 from the waveform, applies the
@@ -531,6 +602,17 @@ int nrse_ccc_loss(const float* pred, int ld, const float* target, float* loss, f
 int nrse_sumsq(const float* x, long long n, double* out, double* part, void* stream);
 /* part (optional): f64 workspace of 4096 doubles; the per-workgroup sums are then added in a
  * fixed order (deterministic) instead of by f64 atomics */
+/* The gradient norm over many tensors and clipping by it (torch.nn.utils.clip_grad_norm_, 2-norm):
+ *   norm[0] = sqrt(sum x^2);  clip: x *= min(1, max_norm / (norm + 1e-6)), in place.
+ * ptrs, numel, dtypes (NRSE_F32 or NRSE_BF16): HOST arrays of `count` contiguous device tensors, any
+ * alignment their type allows; read before the call returns. part: nrse_grad_norm_workspace(...)
+ * doubles. f64 sums in a fixed order. Clipping refuses tensors that overlap, and writes nothing where
+ * the factor is 1; a NaN norm makes every value NaN. */
+long long nrse_grad_norm_workspace(const void* const* ptrs, const long long* numel, const int* dtypes, int count);
+int nrse_grad_norm(const void* const* ptrs, const long long* numel, const int* dtypes, int count, float* norm,
+                   double* part, void* stream);
+int nrse_clip_grad_norm(const void* const* ptrs, const long long* numel, const int* dtypes, int count, double max_norm,
+                        float* norm, double* part, void* stream);
 typedef struct {
   uint32_t struct_size;  /* ABI 10: sizeof(nrse_adamw_params), checked by every entry point taking it */
   float* p; const float* g; float* m; float* v; void* p_shadow; int shadow_dtype;

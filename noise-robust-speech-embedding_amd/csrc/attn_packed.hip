@@ -1,0 +1,1089 @@
+// Attention over packed sequences: rows of all sequences one behind another (or each sequence in its
+// own padded stretch), grouped heads, full or causal, with an optional gated relative-position bias.
+// For row i and key j of one sequence, query head h, key head h / G:
+//   s_ij = scale q_i.k_j + g_i b[j - i]      P = softmax_j(s)      o_i = sum_j P_ij v_j
+//   dV_j = sum_i P_ij dO_i   dP_ij = dO_i.v_j   dS = P (dP - delta_i), delta_i = sum_j P_ij dP_ij
+//   dQ_i = scale sum_j dS_ij k_j   dK_j = scale sum_i dS_ij q_i   (dK, dV summed over the G heads)
+//   dg_i = sum_j dS_ij b[j - i]    db[d] = sum over j - i = d of g_i dS_ij
+//
+// One workgroup = 4 waves = 128 rows (forward, dQ: queries; dK/dV: keys) of one sequence and head;
+// one wave = 32 rows on the 32x32 matrix instructions, whose operand of 32 columns is the wave's own
+// rows: S^T = K Q^T, so a softmax row is one lane and its neighbour 32 lanes on, and the
+// probabilities leave the accumulators as the next product's operand without a shuffle (its inner
+// index is taken in the accumulators' order: key 8 (r / 4) + 4 half + r % 4 for register r). The
+// other side streams through LDS in tiles of 64 rows (32 at 512 bytes a row) by LDS-DMA, one tile ahead.
+// A row of 32 queries per wave reads each K and V tile once for 32 columns: LDS reads
+// (2 tiles x 4 waves) and matrix cycles are then about even at head_dim 128.
+#include <type_traits>
+
+#include "common.h"
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+constexpr int BQ = 128;       // rows of a workgroup
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float INF = __builtin_huge_valf();
+// Lazy rescaling: a row's probabilities are taken relative to a reference that only moves when a
+// score passes it by more than 2^8; f32 sums hold values up to 2^8 as well as values up to 1.
+constexpr float RESCALE_TAU = 8.f;
+
+NRSE_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T, int D>
+struct Geo {
+  static constexpr int RB = D * (int)sizeof(T);         // bytes of a row
+  static constexpr int PANELS = RB / 128;               // a tile is kept in panels of 128-byte rows
+  static constexpr int KT = RB > 256 ? 32 : 64;         // rows of a streamed tile
+  static constexpr int TILE = KT * RB;                  // bytes of a tile
+  static constexpr int NS = RB / 32;                    // 16-byte fragments of a row per lane half
+  static constexpr int DT = D / 32;                     // 32-wide pieces of the head
+  static constexpr int NT = KT / 32;                    // 32-row pieces of a tile
+  static constexpr int DMA = KT / 8 * PANELS / 4;       // LDS-DMA instructions per wave and tile
+  static constexpr int SEG = 192;                       // bias entries of a workgroup's tile, KT + 127, in 64s
+};
+
+// ---------------------------------------------------------------------------------- LDS tiles
+// Row r of a panel holds its 16-byte chunk c at position c ^ sw(r): eight consecutive rows of one
+// chunk (a b128 row read) and four rows of two chunks (a transposed read) then lie on distinct banks.
+NRSE_DEV int sw(int row) { return ((row >> 1) & 3) << 1; }
+template <int KT>
+NRSE_DEV int loff(int row, int chunk) {
+  return (chunk >> 3) * (KT * 128) + row * 128 + (((chunk & 7) ^ sw(row)) << 4);
+}
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// A lane's places in a tile. Everything but the 16-byte chunk's swizzle is a constant offset from
+// them (a 32-row piece or a panel does not change it), so a read is one of these plus an immediate.
+template <typename T, int D>
+struct Lds {
+  using G = Geo<T, D>;
+  int row[4];  // row m, chunk 2 c + half of a panel, c = 0 .. 3
+  int col[2];  // inner index down the rows: bf16 see rd_col; f32: column m of row 4 half (one entry)
+  NRSE_DEV void init(int lane) {
+    const int m = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) row[c] = loff<G::KT>(m, 2 * c + half);
+    if constexpr (std::is_same_v<T, bf16_t>) {
+      const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        col[e] = loff<G::KT>(4 * (g >> 1) + (i >> 2), 4 * e + 2 * (g & 1) + ((i & 3) >> 1)) + (i & 1) * 8;
+    } else {
+      col[0] = col[1] = 0;
+    }
+  }
+  // 16 bytes of row 32 t + m, fragment c
+  NRSE_DEV u32x4 rd_row(const char* tile, int t, int c) const {
+    return *reinterpret_cast<const u32x4*>(tile + row[c & 3] + (c >> 2) * (G::KT * 128) + 32 * t * 128);
+  }
+  // bf16 operand with its inner index down the rows: lane (m, half) gets column 32 dt + m of rows
+  // r0 + 4 half .. + 3 and r0 + 8 + 4 half .. + 3 (r0 a multiple of 16: the swizzle repeats every 8 rows)
+  NRSE_DEV bf16x8 rd_col(const char* tile, int r0, int dt) const {
+    const char* a = tile + col[dt & 1] + (dt >> 1) * (G::KT * 128) + r0 * 128;
+    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)a);
+    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(a + 8 * 128));
+    const short8v v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(bf16x8, v);
+  }
+};
+
+NRSE_DEV bf16x8 pack8(const float* a) {
+  bf16x8 v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (__bf16)a[j];
+  return v;
+}
+
+// acc += A B over one 16-byte fragment of the inner index (8 bf16 or 4 f32 per lane half)
+template <typename T>
+NRSE_DEV void mma_row(u32x4 a, u32x4 b, f32x16& acc) {
+  if constexpr (std::is_same_v<T, bf16_t>) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[c]), __uint_as_float(b[c]), acc, 0, 0, 0);
+  }
+}
+
+// acc[dt] += X^T P for a 32-row piece of the tile at `t` (rows r0 ..): X^T from the tile, P the 16
+// registers of a 32x32 accumulator (rounded to bf16 for the bf16 product: relative 2^-9 per
+// probability, as every bf16 operand)
+template <typename T, int D>
+NRSE_DEV void mma_col(const Lds<T, D>& L, const char* t, int r0, const float* p, f32x16* acc, int lane) {
+  using G = Geo<T, D>;
+  if constexpr (std::is_same_v<T, bf16_t>) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const bf16x8 b = pack8(p + 8 * ks);
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt)
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(L.rd_col(t, r0 + 16 * ks, dt), b, acc[dt], 0, 0, 0);
+    }
+  } else {
+    const int m = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = r0 + 8 * (r >> 2) + 4 * half + (r & 3);
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt) {
+        const float a = *reinterpret_cast<const float*>(t + loff<G::KT>(row, 8 * dt + (m >> 2)) + (m & 3) * 4);
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[dt], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------- LDS-DMA
+// A wave instruction moves 8 rows of a panel (1 KiB): lane l brings row l / 8, position l % 8, that is
+// the logical chunk (l % 8) ^ sw(row), so the swizzle goes into the source address. The descriptor
+// is made per tile (64-bit base: a long sequence's rows pass 32 bits of offset) and ends behind the
+// tile's last row of the sequence: rows past the end land as zeros and nothing behind them is read.
+template <typename T, int D>
+struct Dma {
+  using G = Geo<T, D>;
+  const char* base;   // row 0 of the sequence
+  long long ld;       // bytes between rows
+  int len;
+  unsigned voff;
+  NRSE_DEV void init(const void* p, long long ld_elems, int len_, int lane) {
+    base = (const char*)p;
+    ld = ld_elems * (long long)sizeof(T);
+    len = len_;
+    const int row = lane >> 3;
+    voff = (unsigned)row * (unsigned)ld + (unsigned)(((lane & 7) ^ sw(row)) << 4);
+  }
+  // head: byte offset of the head
+  NRSE_DEV void issue(char* tile, int row0, int wave, long long head = 0) const {
+    const int n = min(G::KT, len - row0);
+    const unsigned ldu = (unsigned)ld;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(base + head + (long long)row0 * ld), 0, n > 0 ? (int)((unsigned)(n - 1) * ldu + G::RB) : 0, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < G::DMA; ++j) {
+      const int k = wave * G::DMA + j;
+      const int panel = k % G::PANELS, rg = k / G::PANELS;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(tile + panel * (G::KT * 128) + rg * 1024), 16,
+                                               voff + (unsigned)(rg * 8) * ldu + (unsigned)(panel * 128), 0, 0, 0);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------------- which rows
+// The blocks of all sequences are numbered from the last sequence's last block down: under a causal
+// mask a block's work grows with its place, so the long ones of a sequence go first. The grid is
+// sized from what the host knows, rows / BQ + sequences, and what is left over ends at once.
+// Bounds are taken from cu_seqlens as they stand in device memory, clamped to the tensors.
+struct Block { int seq0, len, row0; bool any; };
+
+NRSE_DEV Block find_block(const int* __restrict__ cu, const int* __restrict__ used, int nseq, int rows, int want) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int base = 0; base < nseq; base += 64) {
+    const int s = nseq - 1 - (base + lane);
+    int start = 0, len = 0;
+    if (s >= 0) {
+      start = min(max(cu[s], 0), rows);
+      len = min(max(cu[s + 1], start), rows) - start;
+      if (used) len = min(len, max(used[s], 0));
+    }
+    const int nb = (len + BQ - 1) / BQ;
+    int incl = nb;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += up;
+    }
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(before + incl > want);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      const int first = before + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(nb, l);
+      const int n = __builtin_amdgcn_readlane(nb, l);
+      return Block{__builtin_amdgcn_readlane(start, l), __builtin_amdgcn_readlane(len, l),
+                   (n - 1 - (want - first)) * BQ, true};
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return Block{0, 0, 0, false};
+}
+
+// Workgroup i runs on XCD i % 8 (each with its own L2): the XCDs share out the key heads, and where
+// there are fewer than 8 the blocks, so that the G query heads of a block and the blocks of a sequence
+// meet the same K and V in one L2.
+struct Place { int block, kvh, g; };
+__host__ __device__ inline int gcd8(int n) { return (n & 7) == 0 ? 8 : (n & 3) == 0 ? 4 : (n & 1) == 0 ? 2 : 1; }
+NRSE_DEV Place place(int nblk, int hkv, int G) {
+  const int gc = gcd8(hkv), nsub = 8 / gc;
+  const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+  const int per = (nblk + nsub - 1) / nsub * G;
+  const int r = local % per;
+  return Place{(r / G) * nsub + xcd / gc, (xcd % gc) * (hkv / gc) + local / per, r % G};
+}
+inline long long grid_size(long long nblk, int hkv, int G) {
+  const int gc = gcd8(hkv), nsub = 8 / gc;
+  return 8LL * ((nblk + nsub - 1) / nsub) * G * (hkv / gc);
+}
+
+// ---------------------------------------------------------------------------------- the bias
+// The entries of the Toeplitz vector that a workgroup's tile touches, as 4 copies shifted by 0 .. 3, so
+// that a lane's 4 consecutive entries are one aligned 16-byte read; copy s is rotated by 16 s floats
+// inside 64-float blocks, which puts the copies' equal places on different banks.
+NRSE_DEV int bv_pos(int j, int s) { return (j & ~63) | ((j + 16 * s) & 63); }
+template <int SEG>
+NRSE_DEV void bv_store(float* bv, int tid, float v) {
+  if (tid < SEG) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (tid >= s) bv[s * SEG + bv_pos(tid - s, s)] = v;
+  }
+}
+NRSE_DEV float bv_load(const float* __restrict__ vec, int nd, int e) {
+  const float v = vec[min(max(e, 0), nd - 1)];
+  return (e >= 0 && e < nd) ? v : 0.f;
+}
+
+template <typename T>
+NRSE_DEV void store4(T* p, float a, float b, float c, float d) {
+  if constexpr (std::is_same_v<T, bf16_t>) {
+    uint2 u;
+    u.x = (uint32_t)f2bf(a) | ((uint32_t)f2bf(b) << 16);
+    u.y = (uint32_t)f2bf(c) | ((uint32_t)f2bf(d) << 16);
+    *reinterpret_cast<uint2*>(p) = u;
+  } else {
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+  }
+}
+
+NRSE_DEV void wait_all_and_meet() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------------- forward
+template <typename T, int D, bool BIAS, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_params p) {
+  using G = Geo<T, D>;
+  constexpr int KT = G::KT;
+  extern __shared__ __attribute__((aligned(16))) char dyn[];
+  float* const bv0 = reinterpret_cast<float*>(dyn + 4 * G::TILE);  // [2][4][SEG]
+  const int group = p.hq / p.hkv;
+  const int nblk = (int)(p.rows / BQ) + p.nseq;
+  const Place pl = place(nblk, p.hkv, group);
+  if (pl.block >= nblk) return;
+  const Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
+  if (!bl.any) return;
+  const int h = pl.kvh * group + pl.g, len = bl.len;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 31, half = lane >> 5;
+  Lds<T, D> L;
+  L.init(lane);
+  const int q0 = bl.row0 + w * 32;       // this wave's first row in the sequence
+  const int qi = q0 + m;
+  const bool live = q0 < len;            // a wave past the end keeps its share of the copies and the barriers
+  Dma<T, D> kd, vd;
+  kd.init((const T*)p.k + (long long)bl.seq0 * p.k_row + pl.kvh * p.k_head, p.k_row, len, lane);
+  vd.init((const T*)p.v + (long long)bl.seq0 * p.v_row + pl.kvh * p.v_head, p.v_row, len, lane);
+  const int kend = CAUSAL ? min(len, bl.row0 + BQ) : len;
+  const int ntiles = (kend + KT - 1) / KT;
+  kd.issue(dyn, 0, w);
+  vd.issue(dyn + G::TILE, 0, w);
+  const int nd = 2 * p.bias_len - 1;
+  const float* vec = BIAS ? p.bias_vec + (long long)h * nd : nullptr;
+  // segment entry j of the tile at key kb: b[kb - row0 + j - 127]
+  const int e0 = p.bias_len - 1 - bl.row0 - 127;
+  float bnext = 0.f;
+  if constexpr (BIAS) bv_store<G::SEG>(bv0, tid, bv_load(vec, nd, e0 + tid));
+  u32x4 qf[G::NS];
+  const int qc = min(qi, len - 1);       // loads from a row that is there, zeroed after
+  const T* qrow = (const T*)p.q + (long long)(bl.seq0 + qc) * p.q_row + h * p.q_head;
+#pragma unroll
+  for (int s = 0; s < G::NS; ++s) {
+    qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qrow) + (2 * s + half) * 16);
+    if (qi >= len) qf[s] = u32x4{0, 0, 0, 0};
+  }
+  const float c1 = p.scale * LOG2E;
+  float gl = LOG2E;
+  if constexpr (BIAS) {
+    if (p.gate) gl = p.gate[h * p.rows + bl.seq0 + qc] * LOG2E;
+  }
+  const int u0 = 4 * half + 127 - (w * 32 + m);
+  const float* const bcopy = bv0 + (u0 & 3) * G::SEG;
+  const int uj = u0 - (u0 & 3), us = u0 & 3;
+
+  float mref = 0.f, thr = -INF, lsum = 0.f;
+  f32x16 o[G::DT];
+#pragma unroll
+  for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+
+  auto tile = [&](const int it, auto masked_c) {
+    constexpr bool MASKED = decltype(masked_c)::value;
+    const int kb = it * KT;
+    char* const Kt = dyn + (it & 1) * 2 * G::TILE;
+    char* const Vt = Kt + G::TILE;
+    wait_all_and_meet();
+    float4 bb[G::NT][4];
+    if constexpr (BIAS) {
+      // this tile's entries before the next tile's copies are issued (the compiler cannot tell the LDS
+      // that they write from what is read here, and would wait for them)
+#pragma unroll
+      for (int t = 0; t < G::NT; ++t)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          bb[t][a] = *reinterpret_cast<const float4*>(bcopy + (it & 1) * 4 * G::SEG + bv_pos(uj + 32 * t + 8 * a, us));
+    }
+    if (it + 1 < ntiles) {
+      char* const Kn = dyn + ((it + 1) & 1) * 2 * G::TILE;
+      kd.issue(Kn, kb + KT, w);
+      vd.issue(Kn + G::TILE, kb + KT, w);
+      if constexpr (BIAS) bnext = bv_load(vec, nd, e0 + kb + KT + tid);
+    }
+    if (live && (!CAUSAL || kb <= q0 + 31)) {
+      float v[G::NT][16];
+#pragma unroll
+      for (int t = 0; t < G::NT; ++t) {
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < G::NS; ++c) mma_row<T>(L.rd_row(Kt, t, c), qf[c], s);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          if constexpr (BIAS) {
+            v[t][4 * a + 0] = fmaf(s[4 * a + 0], c1, fmaf(gl, bb[t][a].x, -mref));
+            v[t][4 * a + 1] = fmaf(s[4 * a + 1], c1, fmaf(gl, bb[t][a].y, -mref));
+            v[t][4 * a + 2] = fmaf(s[4 * a + 2], c1, fmaf(gl, bb[t][a].z, -mref));
+            v[t][4 * a + 3] = fmaf(s[4 * a + 3], c1, fmaf(gl, bb[t][a].w, -mref));
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[t][4 * a + c] = fmaf(s[4 * a + c], c1, -mref);
+          }
+        }
+      }
+      if constexpr (MASKED) {
+        // keys past the end or, under the causal mask, behind the query
+        const int last = CAUSAL ? min(len - 1, qi) : len - 1;
+#pragma unroll
+        for (int t = 0; t < G::NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            v[t][r] = kb + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) <= last ? v[t][r] : -INF;
+      }
+      float mx = v[0][0];
+#pragma unroll
+      for (int t = 0; t < G::NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, v[t][r]);
+      mx = xor32_max(mx);
+      // thr: RESCALE_TAU once the row has a reference, -inf until then (a row whose bias is -inf
+      // so far has none)
+      if (__builtin_amdgcn_ballot_w64(mx > thr)) {
+        const bool first = thr < 0.f;
+        const float sh = first ? (mx > -INF ? mx : 0.f) : fmaxf(mx, 0.f);
+        const float al = first ? 1.f : exp2_(-sh);
+        thr = mx > -INF ? RESCALE_TAU : thr;
+        mref += sh;
+        lsum *= al;
+#pragma unroll
+        for (int t = 0; t < G::NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) v[t][r] -= sh;
+#pragma unroll
+        for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= al;
+      }
+#pragma unroll
+      for (int t = 0; t < G::NT; ++t) {
+        float part = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          v[t][r] = exp2_(v[t][r]);
+          part += v[t][r];
+        }
+        lsum += part;
+        mma_col<T, D>(L, Vt, 32 * t, v[t], o, lane);
+      }
+    }
+    if constexpr (BIAS) {
+      if (it + 1 < ntiles) bv_store<G::SEG>(bv0 + ((it + 1) & 1) * 4 * G::SEG, tid, bnext);
+    }
+  };
+  // tiles that every row of the workgroup sees whole, then those with a mask
+  const int nfull = min(len, CAUSAL ? bl.row0 + 1 : len) / KT;
+  for (int it = 0; it < nfull; ++it) tile(it, std::false_type{});
+  for (int it = nfull; it < ntiles; ++it) tile(it, std::true_type{});
+
+  const float l = xor32_sum(lsum);
+  if (qi >= len) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row whose bias leaves nothing: zeros
+  T* const orow = (T*)p.out + (long long)(bl.seq0 + qi) * p.out_row + h * p.out_head + 4 * half;
+#pragma unroll
+  for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      store4<T>(orow + 32 * dt + 8 * a, o[dt][4 * a] * inv, o[dt][4 * a + 1] * inv, o[dt][4 * a + 2] * inv,
+                o[dt][4 * a + 3] * inv);
+  if (p.lse && half == 0)
+    p.lse[h * p.rows + bl.seq0 + qi] = l == 0.f ? -INF : (mref + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// ---------------------------------------------------------------------------------- backward: dQ, dgate
+// The forward's loop with P rebuilt from lse; also delta_i, which the dK/dV kernel reads after it.
+// Without a bias delta is rowsum(dO O), from the stored output. The gradients of bias and gate are f32
+// outputs, and the rounding of a bf16 O would be all their error: there delta is summed again as
+// sum_j P dP from the f32 accumulators, and dgate = sum P dP b - delta sum P b.
+template <typename T, int D, bool BIAS, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bwd_params p) {
+  using G = Geo<T, D>;
+  constexpr int KT = G::KT;
+  extern __shared__ __attribute__((aligned(16))) char dyn[];
+  float* const bv0 = reinterpret_cast<float*>(dyn + 4 * G::TILE);
+  const int group = p.hq / p.hkv;
+  const int nblk = (int)(p.rows / BQ) + p.nseq;
+  const Place pl = place(nblk, p.hkv, group);
+  if (pl.block >= nblk) return;
+  const Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
+  if (!bl.any) return;
+  const int h = pl.kvh * group + pl.g, len = bl.len;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 31, half = lane >> 5;
+  Lds<T, D> L;
+  L.init(lane);
+  const int q0 = bl.row0 + w * 32;
+  const int qi = q0 + m;
+  const bool live = q0 < len;
+  Dma<T, D> kd, vd;
+  kd.init((const T*)p.k + (long long)bl.seq0 * p.k_row + pl.kvh * p.k_head, p.k_row, len, lane);
+  vd.init((const T*)p.v + (long long)bl.seq0 * p.v_row + pl.kvh * p.v_head, p.v_row, len, lane);
+  const int kend = CAUSAL ? min(len, bl.row0 + BQ) : len;
+  const int ntiles = (kend + KT - 1) / KT;
+  kd.issue(dyn, 0, w);
+  vd.issue(dyn + G::TILE, 0, w);
+  const int nd = 2 * p.bias_len - 1;
+  const float* vec = BIAS ? p.bias_vec + (long long)h * nd : nullptr;
+  const int e0 = p.bias_len - 1 - bl.row0 - 127;
+  float bnext = 0.f;
+  // (kept finite: P = 0 where the bias is -inf, and 0 * -inf would reach dgate)
+  if constexpr (BIAS) bv_store<G::SEG>(bv0, tid, fmaxf(bv_load(vec, nd, e0 + tid), -3e38f));
+  u32x4 qf[G::NS], df[G::NS];
+  const int qc = min(qi, len - 1);
+  const long long row = bl.seq0 + qc;
+  const char* qrow = (const char*)((const T*)p.q + row * p.q_row + h * p.q_head);
+  const char* drow = (const char*)((const T*)p.dout + row * p.dout_row + h * p.dout_head);
+  const char* orow = (const char*)((const T*)p.out + row * p.out_row + h * p.out_head);
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < G::NS; ++s) {
+    const int at = (2 * s + half) * 16;
+    qf[s] = *reinterpret_cast<const u32x4*>(qrow + at);
+    df[s] = *reinterpret_cast<const u32x4*>(drow + at);
+    u32x4 of = *reinterpret_cast<const u32x4*>(orow + at);
+    if (qi >= len) qf[s] = df[s] = of = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (std::is_same_v<T, bf16_t>)
+        delta += __uint_as_float(df[s][e] << 16) * __uint_as_float(of[e] << 16) +
+                 __uint_as_float(df[s][e] & 0xffff0000u) * __uint_as_float(of[e] & 0xffff0000u);
+      else
+        delta += __uint_as_float(df[s][e]) * __uint_as_float(of[e]);
+    }
+  }
+  delta = xor32_sum(delta);
+  const float c1 = p.scale * LOG2E;
+  float gl = LOG2E;
+  if constexpr (BIAS) {
+    if (p.gate) gl = p.gate[h * p.rows + row] * LOG2E;
+  }
+  float lse2 = p.lse[h * p.rows + row] * LOG2E;
+  if (lse2 == -INF) lse2 = INF;  // nothing left in this row: P = 0
+  const int u0 = 4 * half + 127 - (w * 32 + m);
+  const float* const bcopy = bv0 + (u0 & 3) * G::SEG;
+  const int uj = u0 - (u0 & 3), us = u0 & 3;
+  float sum_pd = 0.f, sum_pb = 0.f, sum_pdb = 0.f;
+  f32x16 dq[G::DT];
+#pragma unroll
+  for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[dt][r] = 0.f;
+
+  auto tile = [&](const int it, auto masked_c) {
+    constexpr bool MASKED = decltype(masked_c)::value;
+    const int kb = it * KT;
+    char* const Kt = dyn + (it & 1) * 2 * G::TILE;
+    char* const Vt = Kt + G::TILE;
+    wait_all_and_meet();
+    float4 bb[G::NT][4];
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int t = 0; t < G::NT; ++t)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          bb[t][a] = *reinterpret_cast<const float4*>(bcopy + (it & 1) * 4 * G::SEG + bv_pos(uj + 32 * t + 8 * a, us));
+    }
+    if (it + 1 < ntiles) {
+      char* const Kn = dyn + ((it + 1) & 1) * 2 * G::TILE;
+      kd.issue(Kn, kb + KT, w);
+      vd.issue(Kn + G::TILE, kb + KT, w);
+      if constexpr (BIAS) bnext = fmaxf(bv_load(vec, nd, e0 + kb + KT + tid), -3e38f);
+    }
+    if (live && (!CAUSAL || kb <= q0 + 31)) {
+      const int last = CAUSAL ? min(len - 1, qi) : len - 1;
+#pragma unroll
+      for (int t = 0; t < G::NT; ++t) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < G::NS; ++c) {
+          mma_row<T>(L.rd_row(Kt, t, c), qf[c], s);
+          mma_row<T>(L.rd_row(Vt, t, c), df[c], dp);
+        }
+        float ds[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float b = 0.f;
+          if constexpr (BIAS) {
+            const float4 b4 = bb[t][r >> 2];
+            b = (r & 3) == 0 ? b4.x : (r & 3) == 1 ? b4.y : (r & 3) == 2 ? b4.z : b4.w;
+          }
+          float e = fmaf(s[r], c1, BIAS ? fmaf(gl, b, -lse2) : -lse2);
+          if constexpr (MASKED) e = kb + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) <= last ? e : -INF;
+          const float pr = exp2_(e);
+          ds[r] = pr * (dp[r] - delta);
+          if constexpr (BIAS) {
+            const float pd = pr * dp[r];
+            sum_pd += pd;
+            sum_pb = fmaf(pr, b, sum_pb);
+            sum_pdb = fmaf(pd, b, sum_pdb);
+          }
+        }
+        mma_col<T, D>(L, Kt, 32 * t, ds, dq, lane);
+      }
+    }
+    if constexpr (BIAS) {
+      if (it + 1 < ntiles) bv_store<G::SEG>(bv0 + ((it + 1) & 1) * 4 * G::SEG, tid, bnext);
+    }
+  };
+  const int nfull = min(len, CAUSAL ? bl.row0 + 1 : len) / KT;
+  for (int it = 0; it < nfull; ++it) tile(it, std::false_type{});
+  for (int it = nfull; it < ntiles; ++it) tile(it, std::true_type{});
+
+  if constexpr (BIAS) {
+    delta = xor32_sum(sum_pd);
+    sum_pb = xor32_sum(sum_pb);
+    sum_pdb = xor32_sum(sum_pdb);
+  }
+  if (qi >= len) return;
+  if (half == 0) {
+    p.delta[h * p.rows + row] = delta;
+    if constexpr (BIAS) {
+      if (p.dgate) p.dgate[h * p.rows + row] = fmaf(-delta, sum_pb, sum_pdb);
+    }
+  }
+  T* const out = (T*)p.dq + row * p.dq_row + h * p.dq_head + 4 * half;
+#pragma unroll
+  for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      store4<T>(out + 32 * dt + 8 * a, dq[dt][4 * a] * p.scale, dq[dt][4 * a + 1] * p.scale, dq[dt][4 * a + 2] * p.scale,
+                dq[dt][4 * a + 3] * p.scale);
+}
+
+// ---------------------------------------------------------------------------------- backward: dK, dV, dbias
+// One workgroup = 128 keys; the queries of every head of the group stream past (their Q and dO tiles by
+// LDS-DMA, lse, delta and gate beside them), so shared heads' gradients are sums in registers, in one
+// order. S = Q K^T here: a lane is a key, its registers 16 queries.
+//
+// dbias: g dS summed along j - i. Register (a, c) of lane (x = lane & 15, kr = (lane >> 4) & 1, half) is
+// query 8 a + 4 half + c and key 16 kr + x: shifted by R = 8 (a & 1) + c lanes inside its row of 16, it
+// joins diagonal 16 kr + x - 4 half - 16 (a >> 1), or, where the shift ran out of the row, the one 16
+// further down. 2 NT + 1 accumulators so hold a tile; all but the last are done with it and go, as 16
+// strips (4 waves x 4 lane rows) of 32 NT, to LDS, where 180 threads of the next iteration add what falls
+// on a diagonal, in one order, into a ring; what the workgroup will not meet again leaves the ring for
+// this block's row of a slab in memory. rows of the slab are added by dbias_kernel: no atomics.
+constexpr int NDIAG = 180;  // diagonals of a 64-query tile: 127 down to -52
+constexpr int RING = 256;
+template <int R>
+NRSE_DEV void diag_add(float v, float& lo, float& hi) {
+  if constexpr (R == 0) {
+    lo += v;
+  } else {
+    lo += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x100 + R, 0xF, 0xF, true));
+    hi += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x110 + 16 - R, 0xF, 0xF, true));
+  }
+}
+__host__ __device__ inline long long slab_row(int bias_len) { return ((bias_len + 63) & ~63) + 192; }
+
+template <typename T, int D, bool BIAS, bool CAUSAL>
+__global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_kernel(const nrse_attn_packed_bwd_params p) {
+  using G = Geo<T, D>;
+  constexpr int KT = G::KT, NT = G::NT;
+  extern __shared__ __attribute__((aligned(16))) char dyn[];
+  float* const rows0 = reinterpret_cast<float*>(dyn + 4 * G::TILE);  // [2][lse, delta, gate][KT]
+  float* const bv0 = rows0 + 6 * KT;                                 // [2][4][SEG]
+  float* const strip0 = bv0 + 8 * G::SEG;                            // [2][16][32 NT]
+  float* const ring = strip0 + 2 * 16 * 32 * NT;                     // [RING]
+  const int group = p.hq / p.hkv;
+  const int nblk = (int)(p.rows / BQ) + p.nseq;
+  const Place pl = place(nblk, p.hkv, 1);
+  if (pl.block >= nblk) return;
+  // a causal block's queries start at its own rows: the first block of a sequence has the most
+  Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const bool dbias = BIAS && p.dbias_vec;
+  int* const meta = dbias ? (int*)p.part + pl.block * 4 : nullptr;
+  if (!bl.any) {
+    if (dbias && tid == 0 && pl.kvh == 0) meta[1] = meta[2] = 0;
+    return;
+  }
+  const int len = bl.len;
+  if (CAUSAL) bl.row0 = (len - 1) / BQ * BQ - bl.row0;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 31, half = lane >> 5;
+  Lds<T, D> L;
+  L.init(lane);
+  const int kb0 = bl.row0, k0 = kb0 + w * 32, kj = k0 + m;
+  const bool live = k0 < len;
+  const int qt0 = CAUSAL ? kb0 / KT : 0, qtn = (len + KT - 1) / KT, nq = qtn - qt0;
+  if (dbias && tid == 0 && pl.kvh == 0) {
+    meta[0] = kb0;
+    meta[1] = qt0 * KT;
+    meta[2] = len + 127;
+  }
+  Dma<T, D> qd, od;
+  qd.init((const T*)p.q + (long long)bl.seq0 * p.q_row, p.q_row, len, lane);
+  od.init((const T*)p.dout + (long long)bl.seq0 * p.dout_row, p.dout_row, len, lane);
+  const int h0 = pl.kvh * group;
+  const int nd = 2 * p.bias_len - 1;
+  float nrow[3] = {INF, 0.f, 1.f}, nbias = 0.f;
+  auto fetch = [&](int h, int qt, int buf) {   // start bringing tile (h, qt) into LDS buffer buf
+    char* const Q = dyn + buf * 2 * G::TILE;
+    qd.issue(Q, qt * KT, w, h * p.q_head * (long long)sizeof(T));
+    od.issue(Q + G::TILE, qt * KT, w, h * p.dout_head * (long long)sizeof(T));
+    if (tid < KT) {
+      const int qi = qt * KT + tid;
+      const long long at = h * p.rows + bl.seq0 + min(qi, len - 1);
+      const float l = p.lse[at], d = p.delta[at];
+      float g = 1.f;
+      if constexpr (BIAS) {
+        if (p.gate) g = p.gate[at];
+      }
+      // rows past the end and rows that were left nothing: P = 0
+      nrow[0] = (qi < len && l != -INF) ? l * LOG2E : INF;
+      nrow[1] = qi < len ? d : 0.f;
+      nrow[2] = qi < len ? g : 1.f;
+    }
+    // segment entry u of the tile: b[kb0 - qb + 127 - u], u = query - key + 127
+    if constexpr (BIAS)
+      nbias = bv_load(p.bias_vec + (long long)h * nd, nd, kb0 - qt * KT + 127 - tid + p.bias_len - 1);
+  };
+  auto keep = [&](int buf) {   // what came by registers
+    if (tid < KT) {
+      float* r = rows0 + buf * 3 * KT + tid;
+      r[0] = nrow[0];
+      r[KT] = nrow[1];
+      r[2 * KT] = nrow[2];
+    }
+    if constexpr (BIAS) bv_store<G::SEG>(bv0 + buf * 4 * G::SEG, tid, nbias);
+  };
+  fetch(h0, qt0, 0);
+  u32x4 kf[G::NS], vf[G::NS];
+  const long long krow = bl.seq0 + min(kj, len - 1);
+  const char* kp = (const char*)((const T*)p.k + krow * p.k_row + pl.kvh * p.k_head);
+  const char* vp = (const char*)((const T*)p.v + krow * p.v_row + pl.kvh * p.v_head);
+#pragma unroll
+  for (int s = 0; s < G::NS; ++s) {
+    kf[s] = *reinterpret_cast<const u32x4*>(kp + (2 * s + half) * 16);
+    vf[s] = *reinterpret_cast<const u32x4*>(vp + (2 * s + half) * 16);
+    if (kj >= len) kf[s] = vf[s] = u32x4{0, 0, 0, 0};
+  }
+  keep(0);
+  const float c1 = p.scale * LOG2E;
+  const int u0 = 4 * half + 127 - (w * 32 + m);
+  const float* const bcopy = bv0 + (u0 & 3) * G::SEG;
+  const int uj = u0 - (u0 & 3), us = u0 & 3;
+  f32x16 dk[G::DT], dv[G::DT];
+#pragma unroll
+  for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[dt][r] = dv[dt][r] = 0.f;
+  float dacc[2 * NT + 1];
+#pragma unroll
+  for (int j = 0; j <= 2 * NT; ++j) dacc[j] = 0.f;
+  float* const mine = strip0 + (w * 4 + (lane >> 4)) * (32 * NT) + (lane & 15) + 16 * (2 * NT - 1);
+  if (dbias) ring[tid] = 0.f;
+
+  // the strips of one tile into the ring; diagonal R is key - query relative to (kb0, qb)
+  auto fold = [&](int buf, int qb, int h, bool end) {
+    const int R = tid + 127 - (NDIAG - 1) + 16 * (3 - (2 * NT - 1));  // 127 down to -4 - 16 (2 NT - 1)
+    if (tid < NDIAG && R <= 127) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int slot = R - 32 * (i >> 2) - 16 * (i & 1) + 4 * ((i >> 1) & 1) + 16 * (2 * NT - 1);
+        const bool in = (unsigned)slot < (unsigned)(32 * NT);
+        const float x = strip0[(buf * 16 + i) * (32 * NT) + (in ? slot : 0)];
+        s += in ? x : 0.f;
+      }
+      const int d = kb0 - qb + R;
+      s += ring[d & (RING - 1)];
+      const bool done = end || R > 127 - KT;
+      ring[d & (RING - 1)] = done ? 0.f : s;
+      const int x = qb + 127 - R;
+      const long long ld = slab_row(p.bias_len);
+      if (done && x < min((int)ld, len + 127))
+        p.part[4LL * nblk + ((long long)h * nblk + pl.block) * ld + x] = s;
+    }
+  };
+  auto shed = [&](int buf) {   // what is done with this tile, to the strips
+#pragma unroll
+    for (int j = 0; j < 2 * NT; ++j) mine[buf * 16 * 32 * NT - 16 * j] = dacc[j];
+    dacc[0] = dacc[2 * NT];
+#pragma unroll
+    for (int j = 1; j <= 2 * NT; ++j) dacc[j] = 0.f;
+  };
+
+  int g = 0, qt = qt0;
+  const int total = group * nq;
+  const bool part_block = kb0 + BQ > len;
+  auto tile = [&](const int it, auto masked_c) {
+    constexpr bool MASKED = decltype(masked_c)::value;
+    const int buf = it & 1, qb = qt * KT;
+    char* const Qt = dyn + buf * 2 * G::TILE;
+    char* const Ot = Qt + G::TILE;
+    const float* const rb = rows0 + buf * 3 * KT + 4 * half;
+    wait_all_and_meet();
+    if (it + 1 < total) {
+      const bool next_head = qt + 1 == qtn;
+      fetch(h0 + g + next_head, next_head ? qt0 : qt + 1, buf ^ 1);
+    }
+    if (dbias && qt > qt0) fold(buf ^ 1, qb - KT, h0 + g, false);
+    if (live && (!CAUSAL || qb + KT - 1 >= k0)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < G::NS; ++c) {
+          mma_row<T>(L.rd_row(Qt, t, c), kf[c], s);
+          mma_row<T>(L.rd_row(Ot, t, c), vf[c], dp);
+        }
+        float pr[16], ds[16];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const float4 l4 = *reinterpret_cast<const float4*>(rb + 32 * t + 8 * a);
+          const float4 d4 = *reinterpret_cast<const float4*>(rb + KT + 32 * t + 8 * a);
+          const float l[4] = {l4.x, l4.y, l4.z, l4.w}, d[4] = {d4.x, d4.y, d4.z, d4.w};
+          float gg[4], b[4];
+          if constexpr (BIAS) {
+            const float4 g4 = *reinterpret_cast<const float4*>(rb + 2 * KT + 32 * t + 8 * a);
+            const float4 b4 = *reinterpret_cast<const float4*>(bcopy + buf * 4 * G::SEG + bv_pos(uj + 32 * t + 8 * a, us));
+            gg[0] = g4.x; gg[1] = g4.y; gg[2] = g4.z; gg[3] = g4.w;
+            b[0] = b4.x; b[1] = b4.y; b[2] = b4.z; b[3] = b4.w;
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int r = 4 * a + c;
+            float e = fmaf(s[r], c1, BIAS ? fmaf(gg[c] * LOG2E, b[c], -l[c]) : -l[c]);
+            if constexpr (MASKED) {
+              const int qi = qb + 32 * t + 8 * a + 4 * half + c;
+              e = (kj < len && (!CAUSAL || kj <= qi)) ? e : -INF;
+            }
+            pr[r] = exp2_(e);
+            ds[r] = pr[r] * (dp[r] - d[c]);
+          }
+          if constexpr (BIAS) {
+            // (a, c): shift 8 (a & 1) + c, accumulator 2 t + (a >> 1)
+            float& lo = dacc[2 * t + (a >> 1)];
+            float& hi = dacc[2 * t + (a >> 1) + 1];
+            if (a & 1) {
+              diag_add<8>(gg[0] * ds[4 * a], lo, hi);
+              diag_add<9>(gg[1] * ds[4 * a + 1], lo, hi);
+              diag_add<10>(gg[2] * ds[4 * a + 2], lo, hi);
+              diag_add<11>(gg[3] * ds[4 * a + 3], lo, hi);
+            } else {
+              diag_add<0>(gg[0] * ds[4 * a], lo, hi);
+              diag_add<1>(gg[1] * ds[4 * a + 1], lo, hi);
+              diag_add<2>(gg[2] * ds[4 * a + 2], lo, hi);
+              diag_add<3>(gg[3] * ds[4 * a + 3], lo, hi);
+            }
+          }
+        }
+        mma_col<T, D>(L, Ot, 32 * t, pr, dv, lane);
+        mma_col<T, D>(L, Qt, 32 * t, ds, dk, lane);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (dbias) shed(buf);
+    if (it + 1 < total) keep(buf ^ 1);
+    if (dbias && qt + 1 == qtn) {
+      // the head's last tile: fold it and the accumulators' rest, and empty the ring
+      __syncthreads();
+      fold(buf, qb, h0 + g, false);
+      __syncthreads();
+      shed(buf);
+      __syncthreads();
+      fold(buf, qb + KT, h0 + g, true);
+#pragma unroll
+      for (int j = 0; j <= 2 * NT; ++j) dacc[j] = 0.f;
+    }
+  };
+  for (int it = 0; it < total; ++it) {
+    if (part_block || (CAUSAL && qt * KT < kb0 + BQ - 1)) tile(it, std::true_type{});
+    else tile(it, std::false_type{});
+    if (++qt == qtn) {
+      qt = qt0;
+      ++g;
+    }
+  }
+  if (kj >= len) return;
+  T* const dko = (T*)p.dk + krow * p.dk_row + pl.kvh * p.dk_head + 4 * half;
+  T* const dvo = (T*)p.dv + krow * p.dv_row + pl.kvh * p.dv_head + 4 * half;
+#pragma unroll
+  for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      store4<T>(dko + 32 * dt + 8 * a, dk[dt][4 * a] * p.scale, dk[dt][4 * a + 1] * p.scale, dk[dt][4 * a + 2] * p.scale,
+                dk[dt][4 * a + 3] * p.scale);
+      store4<T>(dvo + 32 * dt + 8 * a, dv[dt][4 * a], dv[dt][4 * a + 1], dv[dt][4 * a + 2], dv[dt][4 * a + 3]);
+    }
+}
+
+// dbias[h, d] (+)= the slab's rows: for each diagonal, the blocks that hold it, in block order within 4
+// quarters of the blocks, then the quarters in order.
+__global__ __launch_bounds__(256) void dbias_kernel(const float* __restrict__ part, float* __restrict__ dvec, int nblk,
+                                                    int bias_len, int accumulate) {
+  __shared__ float red[4][64];
+  const int nd = 2 * bias_len - 1, h = blockIdx.y;
+  const int e = blockIdx.x * 64 + (threadIdx.x & 63), wv = threadIdx.x >> 6;
+  const int d = e - (bias_len - 1);
+  const int* meta = (const int*)part;
+  const long long ld = slab_row(bias_len);
+  const float* slab = part + 4LL * nblk + (long long)h * nblk * ld;
+  const int per = (nblk + 3) / 4, b0 = wv * per, b1 = min(nblk, b0 + per);
+  float s = 0.f;
+  for (int b = b0; b < b1; ++b) {
+    const int kb = meta[4 * b], x0 = meta[4 * b + 1], x1 = meta[4 * b + 2];
+    const int x = kb + 127 - d;
+    if (x >= x0 && x < x1 && x < ld) s += slab[(long long)b * ld + x];
+  }
+  red[wv][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (wv == 0 && e < nd) {
+    const int i = threadIdx.x;
+    const float v = red[0][i] + red[1][i] + red[2][i] + red[3][i];
+    float* o = dvec + (long long)h * nd + e;
+    *o = accumulate ? *o + v : v;
+  }
+}
+
+// ---------------------------------------------------------------------------------- bias tables
+// bucket of a relative position: the last of `edges` (ascending, edges[0] = 0) that is <= its distance;
+// two-sided (causal = 0): the keys behind the query take the first n buckets, those ahead the next n;
+// causal: all n are the past's, and a key ahead counts as distance 0.
+NRSE_DEV int bucket_of(const int* edges, int n, int rel, int causal) {
+  const int dist = causal ? max(-rel, 0) : abs(rel);
+  int lo = 0, hi = n;  // edges[lo] <= dist < edges[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (edges[mid] <= dist) lo = mid;
+    else hi = mid;
+  }
+  return lo + (!causal && rel > 0 ? n : 0);
+}
+
+__global__ __launch_bounds__(256) void rel_expand_kernel(const float* __restrict__ E, const int* __restrict__ edges, int n,
+                                                         float* __restrict__ vec, int H, int T, int causal) {
+  const int nd = 2 * T - 1;
+  const long long total = (long long)H * nd;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const int h = (int)(i / nd), e = (int)(i - (long long)h * nd);
+    vec[i] = E[(long long)bucket_of(edges, n, e - (T - 1), causal) * H + h];
+  }
+}
+
+// dE[bucket, h] (+)= the sum of dvec[h, d] over the bucket's distances: they are one run of d (two for
+// bucket 0 of a causal table: the keys ahead count as distance 0). One wave per bucket and head, lane
+// sums 64 apart, then a fixed tree.
+__global__ __launch_bounds__(256) void rel_collect_kernel(const float* __restrict__ dvec, const int* __restrict__ edges,
+                                                          int n, float* __restrict__ dE, int H, int T, int causal,
+                                                          int accumulate) {
+  const int nb = causal ? n : 2 * n;
+  const int id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (id >= nb * H) return;
+  const int b = id / H, h = id % H, k = b % n;
+  const bool ahead = b >= n;
+  // distances [edges[k], edges[k + 1]), at most T - 1; none at distance 0 ahead of the query
+  const int d0 = max(edges[k], ahead ? 1 : 0), d1 = min(k + 1 < n ? edges[k + 1] : T, T);
+  const int nd = 2 * T - 1;
+  const float* row = dvec + (long long)h * nd + (T - 1);  // row[j - i]
+  float s = 0.f;
+  for (int d = d0 + lane; d < d1; d += 64) s += row[ahead ? d : -d];
+  if (causal && b == 0)
+    for (int d = 1 + lane; d < T; d += 64) s += row[d];
+  s = wave_sum(s);
+  if (lane == 0) dE[(long long)b * H + h] = accumulate ? dE[(long long)b * H + h] + s : s;
+}
+
+// ---------------------------------------------------------------------------------- launches
+template <typename T, int D>
+size_t lds_fwd(bool bias) { return 4 * Geo<T, D>::TILE + (bias ? 8 * Geo<T, D>::SEG * sizeof(float) : 0); }
+template <typename T, int D>
+size_t lds_kv(bool bias) {
+  using G = Geo<T, D>;
+  return 4 * G::TILE + 6 * G::KT * sizeof(float) +
+         (bias ? (8 * G::SEG + 2 * 16 * 32 * G::NT + RING) * sizeof(float) : 0);
+}
+
+template <typename T, int D, bool BIAS, bool CAUSAL>
+void launch_fwd(const nrse_attn_packed_fwd_params& p, hipStream_t st) {
+  const long long n = grid_size(p.rows / BQ + p.nseq, p.hkv, p.hq / p.hkv);
+  hipLaunchKernelGGL((fwd_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)n), dim3(256), (lds_fwd<T, D>(BIAS)), st, p);
+}
+template <typename T, int D, bool BIAS, bool CAUSAL>
+void launch_bwd(const nrse_attn_packed_bwd_params& p, hipStream_t st) {
+  const long long nblk = p.rows / BQ + p.nseq;
+  hipLaunchKernelGGL((bwd_q_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, p.hq / p.hkv)), dim3(256),
+                     (lds_fwd<T, D>(BIAS)), st, p);
+  hipLaunchKernelGGL((bwd_kv_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, 1)), dim3(256),
+                     (lds_kv<T, D>(BIAS)), st, p);
+}
+
+template <typename P, typename F>
+void dispatch(const P& p, F f) {
+  const bool b = p.bias_vec, c = p.causal;
+  auto with_mask = [&](auto t, auto d, auto bias) {
+    if (c) f(t, d, bias, std::true_type{});
+    else f(t, d, bias, std::false_type{});
+  };
+  auto with_bias = [&](auto t, auto d) {
+    if (b) with_mask(t, d, std::true_type{});
+    else with_mask(t, d, std::false_type{});
+  };
+  using d64 = std::integral_constant<int, 64>;
+  using d128 = std::integral_constant<int, 128>;
+  if (p.dtype == NRSE_BF16) p.head_dim == 64 ? with_bias(bf16_t{}, d64{}) : with_bias(bf16_t{}, d128{});
+  else p.head_dim == 64 ? with_bias(float{}, d64{}) : with_bias(float{}, d128{});
+}
+
+// one operand: 16-byte rows, and no row so far on that 64 of them pass 32 bits of offset
+int check_rows(const char* fn, const char* name, const void* ptr, long long row, long long head, const int dtype, int D,
+               int heads) {
+  const int es = dtype == NRSE_BF16 ? 2 : 4;
+  NRSE_REQUIRE(ptr, "%s: %s is null", fn, name);
+  NRSE_REQUIRE(((uintptr_t)ptr & 15) == 0 && (row * es) % 16 == 0 && (head * es) % 16 == 0,
+               "%s: %s: base and strides (%lld rows, %lld heads) must be 16-byte multiples", fn, name, row, head);
+  NRSE_REQUIRE(row >= D && row * es <= (1 << 24), "%s: %s: row stride %lld outside [head_dim, 2^24 bytes]", fn, name, row);
+  NRSE_REQUIRE(heads == 1 || head >= D, "%s: %s: head stride %lld below head_dim", fn, name, head);
+  return NRSE_OK;
+}
+
+template <typename P>
+int check_common(const char* fn, const P* p) {
+  NRSE_REQUIRE(p->dtype == NRSE_BF16 || p->dtype == NRSE_F32, "%s: dtype %d (bf16 and f32 only)", fn, p->dtype);
+  NRSE_REQUIRE(p->head_dim == 64 || p->head_dim == 128, "%s: head_dim %d (64 and 128 only)", fn, p->head_dim);
+  NRSE_REQUIRE(p->hkv > 0 && p->hq > 0 && p->hq % p->hkv == 0, "%s: %d query heads over %d key heads", fn, p->hq, p->hkv);
+  NRSE_REQUIRE(p->rows >= 0 && p->rows < (1LL << 31) - 256 && p->nseq >= 0, "%s: rows %lld, sequences %d", fn, p->rows,
+               p->nseq);
+  NRSE_REQUIRE(p->nseq == 0 || p->cu_seqlens, "%s: cu_seqlens is null", fn);
+  NRSE_REQUIRE(!p->bias_vec || (p->bias_len > 0 && p->bias_len <= (1 << 29)), "%s: bias_len %d", fn, p->bias_len);
+  NRSE_REQUIRE(p->bias_vec || !p->gate, "%s: a gate needs a bias", fn);
+  NRSE_REQUIRE(grid_size(p->rows / BQ + p->nseq, p->hkv, p->hq / p->hkv) < (1LL << 31), "%s: too many workgroups", fn);
+  return NRSE_OK;
+}
+#define ROWS(fn, x) \
+  if (const int rc = check_rows(fn, #x, p->x, p->x##_row, p->x##_head, p->dtype, p->head_dim, p->hq)) return rc
+#define ROWS_KV(fn, x) \
+  if (const int rc = check_rows(fn, #x, p->x, p->x##_row, p->x##_head, p->dtype, p->head_dim, p->hkv)) return rc
+
+}  // namespace
+
+extern "C" int nrse_attn_packed_fwd(const nrse_attn_packed_fwd_params* p, void* stream) {
+  const char* fn = "nrse_attn_packed_fwd";
+  NRSE_CHECK_PARAMS(p, fn);
+  if (const int rc = check_common(fn, p)) return rc;
+  if (p->rows == 0 || p->nseq == 0) return NRSE_OK;
+  ROWS(fn, q);
+  ROWS_KV(fn, k);
+  ROWS_KV(fn, v);
+  ROWS(fn, out);
+  dispatch(*p, [&](auto t, auto d, auto b, auto c) {
+    launch_fwd<decltype(t), decltype(d)::value, decltype(b)::value, decltype(c)::value>(*p, (hipStream_t)stream);
+  });
+  return nrse_check_launch(fn);
+}
+
+extern "C" long long nrse_attn_packed_bwd_workspace(const nrse_attn_packed_bwd_params* p) {
+  NRSE_CHECK_PARAMS(p, "nrse_attn_packed_bwd_workspace");
+  if (const int rc = check_common("nrse_attn_packed_bwd_workspace", p)) return rc;
+  if (!p->bias_vec || !p->dbias_vec) return 0;
+  const long long nblk = p->rows / BQ + p->nseq;
+  return nblk * 4 + p->hq * nblk * slab_row(p->bias_len);
+}
+
+extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* stream) {
+  const char* fn = "nrse_attn_packed_bwd";
+  NRSE_CHECK_PARAMS(p, fn);
+  if (const int rc = check_common(fn, p)) return rc;
+  NRSE_REQUIRE(p->bias_vec || (!p->dbias_vec && !p->dgate), "%s: gradients of a bias that is not there", fn);
+  NRSE_REQUIRE(p->gate || !p->dgate, "%s: dgate without a gate", fn);
+  const hipStream_t st = (hipStream_t)stream;
+  if (p->rows == 0 || p->nseq == 0) {
+    if (p->dbias_vec && !p->accumulate) {
+      const long long n = (long long)p->hq * (2LL * p->bias_len - 1);
+      return nrse_zero(p->dbias_vec, n, stream);
+    }
+    return NRSE_OK;
+  }
+  ROWS(fn, q);
+  ROWS_KV(fn, k);
+  ROWS_KV(fn, v);
+  ROWS(fn, out);
+  ROWS(fn, dout);
+  ROWS(fn, dq);
+  ROWS_KV(fn, dk);
+  ROWS_KV(fn, dv);
+  NRSE_REQUIRE(p->lse && p->delta, "%s: lse and delta are needed", fn);
+  NRSE_REQUIRE(!p->dbias_vec || p->part, "%s: dbias_vec needs the workspace (nrse_attn_packed_bwd_workspace)", fn);
+  dispatch(*p, [&](auto t, auto d, auto b, auto c) {
+    launch_bwd<decltype(t), decltype(d)::value, decltype(b)::value, decltype(c)::value>(*p, st);
+  });
+  if (p->dbias_vec) {
+    const int nd = 2 * p->bias_len - 1;
+    hipLaunchKernelGGL(dbias_kernel, dim3((nd + 63) / 64, p->hq), dim3(256), 0, st, p->part, p->dbias_vec,
+                       (int)(p->rows / BQ) + p->nseq, p->bias_len, p->accumulate);
+  }
+  return nrse_check_launch(fn);
+}
+
+extern "C" int nrse_rel_bias_expand(const float* E, const int* edges, int n, float* vec, int H, int T, int causal,
+                                    void* stream) {
+  NRSE_REQUIRE(E && edges && vec && n > 0 && H > 0 && T > 0 && T <= (1 << 29), "nrse_rel_bias_expand: bad args");
+  const long long total = (long long)H * (2LL * T - 1);
+  const long long blocks = (total + 255) / 256;
+  hipLaunchKernelGGL(rel_expand_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0,
+                     (hipStream_t)stream, E, edges, n, vec, H, T, causal);
+  return nrse_check_launch("nrse_rel_bias_expand");
+}
+
+extern "C" int nrse_rel_bias_collect(const float* dvec, const int* edges, int n, float* dE, int H, int T, int causal,
+                                     int accumulate, void* stream) {
+  NRSE_REQUIRE(dvec && edges && dE && n > 0 && H > 0 && T > 0 && T <= (1 << 29), "nrse_rel_bias_collect: bad args");
+  const long long items = (long long)(causal ? n : 2 * n) * H;
+  NRSE_REQUIRE(items < (1LL << 31), "nrse_rel_bias_collect: %lld table entries", items);
+  hipLaunchKernelGGL(rel_collect_kernel, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, (hipStream_t)stream, dvec, edges,
+                     n, dE, H, T, causal, accumulate);
+  return nrse_check_launch("nrse_rel_bias_collect");
+}

@@ -110,6 +110,27 @@ class AttnBwdParams(_Sized):
                 ("dropout_p", c_f), ("seed", c_u32), ("bias_vec", c_vp), ("diag_part", c_vp), ("drop_mask", c_vp)]
 
 
+_STRIDES = ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row", "out_head")
+
+
+class AttnPackedFwdParams(_Sized):
+    _fields_ = [("struct_size", c_u32), ("dtype", c_int), ("q", c_vp), ("k", c_vp), ("v", c_vp), ("out", c_vp),
+                *((s, c_ll) for s in _STRIDES), ("lse", c_vp), ("cu_seqlens", c_vp), ("seq_lens", c_vp),
+                ("nseq", c_int), ("causal", c_int), ("rows", c_ll), ("hq", c_int), ("hkv", c_int),
+                ("head_dim", c_int), ("scale", c_f), ("bias_vec", c_vp), ("gate", c_vp), ("bias_len", c_int)]
+
+
+class AttnPackedBwdParams(_Sized):
+    _fields_ = [("struct_size", c_u32), ("dtype", c_int), ("q", c_vp), ("k", c_vp), ("v", c_vp), ("out", c_vp),
+                ("dout", c_vp), ("dq", c_vp), ("dk", c_vp), ("dv", c_vp), *((s, c_ll) for s in _STRIDES),
+                *((s, c_ll) for s in ("dout_row", "dout_head", "dq_row", "dq_head", "dk_row", "dk_head", "dv_row",
+                                      "dv_head")),
+                ("lse", c_vp), ("delta", c_vp), ("cu_seqlens", c_vp), ("seq_lens", c_vp), ("nseq", c_int),
+                ("causal", c_int), ("rows", c_ll), ("hq", c_int), ("hkv", c_int), ("head_dim", c_int),
+                ("scale", c_f), ("bias_vec", c_vp), ("gate", c_vp), ("bias_len", c_int), ("accumulate", c_int),
+                ("dgate", c_vp), ("dbias_vec", c_vp), ("part", c_vp)]
+
+
 class Conv0Params(_Sized):
     _fields_ = [("struct_size", c_u32), ("wav", c_vp), ("L", c_int), ("w", c_vp), ("gamma", c_vp), ("beta", c_vp), ("out", c_vp),
                 ("out_dtype", c_int), ("mean", c_vp), ("rstd", c_vp),
@@ -160,6 +181,11 @@ _SIGNATURES = {
     "nrse_attn_bwd": ([_P(AttnBwdParams), c_vp], c_int),
     "nrse_attn_bwd_workspace": ([_P(AttnBwdParams)], c_ll),
     "nrse_attn_mask_elems": ([c_int, c_int, c_int], c_ll),
+    "nrse_attn_packed_fwd": ([_P(AttnPackedFwdParams), c_vp], c_int),
+    "nrse_attn_packed_bwd": ([_P(AttnPackedBwdParams), c_vp], c_int),
+    "nrse_attn_packed_bwd_workspace": ([_P(AttnPackedBwdParams)], c_ll),
+    "nrse_rel_bias_expand": ([c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int, c_vp], c_int),
+    "nrse_rel_bias_collect": ([c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int, c_int, c_vp], c_int),
     "nrse_conv0_fwd": ([_P(Conv0Params), c_vp], c_int),
     "nrse_conv0_bwd": ([_P(Conv0Params), c_vp], c_int),
     "nrse_conv0_bwd_workspace": ([_P(Conv0Params)], c_ll),
@@ -196,6 +222,9 @@ _SIGNATURES = {
                             c_int, c_vp], c_int),
     "nrse_byol_loss": ([c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_f, c_vp, c_vp], c_int),
     "nrse_sumsq": ([c_vp, c_ll, c_vp, c_vp, c_vp], c_int),
+    "nrse_grad_norm_workspace": ([c_vp, c_vp, c_vp, c_int], c_ll),
+    "nrse_grad_norm": ([c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp], c_int),
+    "nrse_clip_grad_norm": ([c_vp, c_vp, c_vp, c_int, ctypes.c_double, c_vp, c_vp, c_vp], c_int),
     "nrse_adamw": ([_P(AdamWParams), c_vp], c_int),
     "nrse_ema": ([c_vp, c_vp, c_vp, c_int, c_ll, c_f, c_vp, c_vp], c_int),
     "nrse_health": ([c_vp, c_int, c_ll, c_vp, c_vp], c_int),

@@ -42,6 +42,25 @@ def bucket_runs(bucket: np.ndarray, nb: int) -> tuple[np.ndarray, np.ndarray]:
     return order, offsets
 
 
+def bucket_edges(num_buckets: int = 320, max_distance: int = 800, causal: bool = False) -> np.ndarray:
+    """int32 [n]: the smallest distance of each bucket of one side, ascending from 0 (n = num_buckets / 2 two-sided,
+    num_buckets causal): bucket_vector's buckets as borders, for rel_bias_expand / rel_bias_collect. A bucket that
+    no distance falls in repeats its successor's border (or, at the top, ends past every length)."""
+    n = num_buckets if causal else num_buckets // 2
+    if n < 2 or max_distance <= n // 2:
+        raise ValueError(f"{num_buckets} buckets up to distance {max_distance}")
+    max_exact = n // 2
+    rp = np.arange(max_distance + 2, dtype=np.int64)
+    with np.errstate(divide="ignore"):
+        lg = np.log(rp.astype(np.float32) / np.float32(max_exact)).astype(np.float32)
+    lg = (lg / np.float32(math.log(max_distance / max_exact))).astype(np.float32)
+    lg = (lg * np.float32(n - max_exact)).astype(np.float32)
+    large = np.minimum(max_exact + np.where(np.isfinite(lg), lg, 0).astype(np.int64), n - 1)
+    of = np.where(rp < max_exact, rp, large)
+    edges = np.searchsorted(of, np.arange(n), side="left")
+    return np.where(edges > max_distance + 1, np.iinfo(np.int32).max, edges).astype(np.int32)
+
+
 def compute_mask_indices(rng: np.random.Generator, batch: int, T: int, mask_prob: float, mask_length: int,
                          min_masks: int = 0) -> np.ndarray:
     """SpecAugment time masks with the reference's span algorithm (no attention mask: every
