@@ -378,8 +378,8 @@ typedef struct {
 
 /* dq, dk, dv are overwritten (dk, dv: summed over the query heads that share a key head, in one
  * order). delta [hq, rows]: scratch. dgate [hq, rows] (optional, with a gate). dbias_vec (optional, with
- * a bias): d(loss)/d(bias_vec), overwritten, or added to if accumulate; needs part, a workspace of
- * nrse_attn_packed_bwd_workspace(p) floats. No atomics: the same inputs give the same bits. */
+ * a bias): d(loss)/d(bias_vec), overwritten, or added to if accumulate. part: a workspace of
+ * nrse_attn_packed_bwd_workspace(p) floats (NULL where that is 0), 16-byte aligned. No atomics: the same inputs give the same bits. */
 typedef struct {
   uint32_t struct_size;
   int dtype;

@@ -14,6 +14,7 @@
 // other side streams through LDS in tiles of 64 rows (32 at 512 bytes a row) by LDS-DMA, one tile ahead.
 // A row of 32 queries per wave reads each K and V tile once for 32 columns: LDS reads
 // (2 tiles x 4 waves) and matrix cycles are then about even at head_dim 128.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -34,11 +35,12 @@ constexpr float RESCALE_TAU = 8.f;
 
 NRSE_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <typename T, int D>
+constexpr int tile_rows(int row_bytes) { return row_bytes > 256 ? 32 : 64; }
+template <typename T, int D, int KT_ = tile_rows(D * (int)sizeof(T))>
 struct Geo {
   static constexpr int RB = D * (int)sizeof(T);         // bytes of a row
   static constexpr int PANELS = RB / 128;               // a tile is kept in panels of 128-byte rows
-  static constexpr int KT = RB > 256 ? 32 : 64;         // rows of a streamed tile
+  static constexpr int KT = KT_;                        // rows of a streamed tile
   static constexpr int TILE = KT * RB;                  // bytes of a tile
   static constexpr int NS = RB / 32;                    // 16-byte fragments of a row per lane half
   static constexpr int DT = D / 32;                     // 32-wide pieces of the head
@@ -60,9 +62,8 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // A lane's places in a tile. Everything but the 16-byte chunk's swizzle is a constant offset from
 // them (a 32-row piece or a panel does not change it), so a read is one of these plus an immediate.
-template <typename T, int D>
+template <typename T, typename G>
 struct Lds {
-  using G = Geo<T, D>;
   int row[4];  // row m, chunk 2 c + half of a panel, c = 0 .. 3
   int col[2];  // inner index down the rows: bf16 see rd_col; f32: column m of row 4 half (one entry)
   NRSE_DEV void init(int lane) {
@@ -115,9 +116,8 @@ NRSE_DEV void mma_row(u32x4 a, u32x4 b, f32x16& acc) {
 // acc[dt] += X^T P for a 32-row piece of the tile at `t` (rows r0 ..): X^T from the tile, P the 16
 // registers of a 32x32 accumulator (rounded to bf16 for the bf16 product: relative 2^-9 per
 // probability, as every bf16 operand)
-template <typename T, int D>
-NRSE_DEV void mma_col(const Lds<T, D>& L, const char* t, int r0, const float* p, f32x16* acc, int lane) {
-  using G = Geo<T, D>;
+template <typename T, typename G>
+NRSE_DEV void mma_col(const Lds<T, G>& L, const char* t, int r0, const float* p, f32x16* acc, int lane) {
   if constexpr (std::is_same_v<T, bf16_t>) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -145,9 +145,8 @@ NRSE_DEV void mma_col(const Lds<T, D>& L, const char* t, int r0, const float* p,
 // the logical chunk (l % 8) ^ sw(row), so the swizzle goes into the source address. The descriptor
 // is made per tile (64-bit base: a long sequence's rows pass 32 bits of offset) and ends behind the
 // tile's last row of the sequence: rows past the end land as zeros and nothing behind them is read.
-template <typename T, int D>
+template <typename T, typename G>
 struct Dma {
-  using G = Geo<T, D>;
   const char* base;   // row 0 of the sequence
   long long ld;       // bytes between rows
   int len;
@@ -283,12 +282,12 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 31, half = lane >> 5;
-  Lds<T, D> L;
+  Lds<T, G> L;
   L.init(lane);
   const int q0 = bl.row0 + w * 32;       // this wave's first row in the sequence
   const int qi = q0 + m;
   const bool live = q0 < len;            // a wave past the end keeps its share of the copies and the barriers
-  Dma<T, D> kd, vd;
+  Dma<T, G> kd, vd;
   kd.init((const T*)p.k + (long long)bl.seq0 * p.k_row + pl.kvh * p.k_head, p.k_row, len, lane);
   vd.init((const T*)p.v + (long long)bl.seq0 * p.v_row + pl.kvh * p.v_head, p.v_row, len, lane);
   const int kend = CAUSAL ? min(len, bl.row0 + BQ) : len;
@@ -411,7 +410,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_
           part += v[t][r];
         }
         lsum += part;
-        mma_col<T, D>(L, Vt, 32 * t, v[t], o, lane);
+        mma_col<T, G>(L, Vt, 32 * t, v[t], o, lane);
       }
     }
     if constexpr (BIAS) {
@@ -458,12 +457,12 @@ __global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bw
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 31, half = lane >> 5;
-  Lds<T, D> L;
+  Lds<T, G> L;
   L.init(lane);
   const int q0 = bl.row0 + w * 32;
   const int qi = q0 + m;
   const bool live = q0 < len;
-  Dma<T, D> kd, vd;
+  Dma<T, G> kd, vd;
   kd.init((const T*)p.k + (long long)bl.seq0 * p.k_row + pl.kvh * p.k_head, p.k_row, len, lane);
   vd.init((const T*)p.v + (long long)bl.seq0 * p.v_row + pl.kvh * p.v_head, p.v_row, len, lane);
   const int kend = CAUSAL ? min(len, bl.row0 + BQ) : len;
@@ -568,7 +567,7 @@ __global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bw
             sum_pdb = fmaf(pd, b, sum_pdb);
           }
         }
-        mma_col<T, D>(L, Kt, 32 * t, ds, dq, lane);
+        mma_col<T, G>(L, Kt, 32 * t, ds, dq, lane);
       }
     }
     if constexpr (BIAS) {
@@ -609,11 +608,10 @@ __global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bw
 // query 8 a + 4 half + c and key 16 kr + x: shifted by R = 8 (a & 1) + c lanes inside its row of 16, it
 // joins diagonal 16 kr + x - 4 half - 16 (a >> 1), or, where the shift ran out of the row, the one 16
 // further down. 2 NT + 1 accumulators so hold a tile; all but the last are done with it and go, as 16
-// strips (4 waves x 4 lane rows) of 32 NT, to LDS, where 180 threads of the next iteration add what falls
-// on a diagonal, in one order, into a ring; what the workgroup will not meet again leaves the ring for
+// strips (4 waves x 4 lane rows) of 32 NT, to LDS, where the next iteration adds what falls on a diagonal,
+// a thread each, in one order, into a ring; what the workgroup will not meet again leaves the ring for
 // this block's row of a slab in memory. rows of the slab are added by dbias_kernel: no atomics.
-constexpr int NDIAG = 180;  // diagonals of a 64-query tile: 127 down to -52
-constexpr int RING = 256;
+constexpr int RING = 192;   // more than the diagonals of a tile
 template <int R>
 NRSE_DEV void diag_add(float v, float& lo, float& hi) {
   if constexpr (R == 0) {
@@ -625,18 +623,27 @@ NRSE_DEV void diag_add(float v, float& lo, float& hi) {
 }
 __host__ __device__ inline long long slab_row(int bias_len) { return ((bias_len + 63) & ~63) + 192; }
 
+template <typename T, int D>
+struct KvGeo : Geo<T, D, (D * sizeof(T) > 128 ? 32 : 64)> {
+  // bf16 at head_dim 128: the accumulators and K fill a wave's 256 registers, V's fragments stay in LDS
+  static constexpr bool VLDS = sizeof(T) == 2 && D == 128;
+  static constexpr int WAVES = sizeof(T) == 4 && D == 128 ? 1 : 2;   // per SIMD
+};
+
 template <typename T, int D, bool BIAS, bool CAUSAL>
-__global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_kernel(const nrse_attn_packed_bwd_params p) {
-  using G = Geo<T, D>;
+__global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const nrse_attn_packed_bwd_params p, int slices,
+                                                                         float* __restrict__ sums) {
+  using G = KvGeo<T, D>;
   constexpr int KT = G::KT, NT = G::NT;
   extern __shared__ __attribute__((aligned(16))) char dyn[];
-  float* const rows0 = reinterpret_cast<float*>(dyn + 4 * G::TILE);  // [2][lse, delta, gate][KT]
+  char* const vt0 = dyn + 4 * G::TILE;                                // [4] tiles of 32 V rows
+  float* const rows0 = reinterpret_cast<float*>(vt0 + (G::VLDS ? 4 * G::TILE : 0));  // [2][lse, delta, gate][KT]
   float* const bv0 = rows0 + 6 * KT;                                 // [2][4][SEG]
   float* const strip0 = bv0 + 8 * G::SEG;                            // [2][16][32 NT]
   float* const ring = strip0 + 2 * 16 * 32 * NT;                     // [RING]
   const int group = p.hq / p.hkv;
   const int nblk = (int)(p.rows / BQ) + p.nseq;
-  const Place pl = place(nblk, p.hkv, 1);
+  const Place pl = place(nblk, p.hkv, slices);
   if (pl.block >= nblk) return;
   // a causal block's queries start at its own rows: the first block of a sequence has the most
   Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
@@ -644,24 +651,24 @@ __global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_ker
   const bool dbias = BIAS && p.dbias_vec;
   int* const meta = dbias ? (int*)p.part + pl.block * 4 : nullptr;
   if (!bl.any) {
-    if (dbias && tid == 0 && pl.kvh == 0) meta[1] = meta[2] = 0;
+    if (dbias && tid == 0 && pl.kvh == 0 && pl.g == 0) meta[1] = meta[2] = 0;
     return;
   }
   const int len = bl.len;
   if (CAUSAL) bl.row0 = (len - 1) / BQ * BQ - bl.row0;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 31, half = lane >> 5;
-  Lds<T, D> L;
+  Lds<T, G> L;
   L.init(lane);
   const int kb0 = bl.row0, k0 = kb0 + w * 32, kj = k0 + m;
   const bool live = k0 < len;
   const int qt0 = CAUSAL ? kb0 / KT : 0, qtn = (len + KT - 1) / KT, nq = qtn - qt0;
-  if (dbias && tid == 0 && pl.kvh == 0) {
+  if (dbias && tid == 0 && pl.kvh == 0 && pl.g == 0) {
     meta[0] = kb0;
     meta[1] = qt0 * KT;
     meta[2] = len + 127;
   }
-  Dma<T, D> qd, od;
+  Dma<T, G> qd, od;
   qd.init((const T*)p.q + (long long)bl.seq0 * p.q_row, p.q_row, len, lane);
   od.init((const T*)p.dout + (long long)bl.seq0 * p.dout_row, p.dout_row, len, lane);
   const int h0 = pl.kvh * group;
@@ -697,18 +704,32 @@ __global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_ker
     }
     if constexpr (BIAS) bv_store<G::SEG>(bv0 + buf * 4 * G::SEG, tid, nbias);
   };
-  fetch(h0, qt0, 0);
-  u32x4 kf[G::NS], vf[G::NS];
+  // this slice's share of the group's (head, query tile) pairs; of whole heads where there is a bias
+  const int total = group * nq;
+  const int it0 = (int)((long long)total * pl.g / slices), it1 = (int)((long long)total * (pl.g + 1) / slices);
+  int g = it0 / nq, qt = qt0 + it0 % nq;
+  if (it0 < it1) fetch(h0 + g, qt, it0 & 1);
+  Dma<T, G> vd;
+  if constexpr (G::VLDS) {
+    vd.init((const T*)p.v + (long long)bl.seq0 * p.v_row + pl.kvh * p.v_head, p.v_row, len, lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vd.issue(vt0 + i * G::TILE, kb0 + 32 * i, w);
+  }
+  const char* const vt = vt0 + w * G::TILE;
+  u32x4 kf[G::NS], vf[G::VLDS ? 1 : G::NS];
   const long long krow = bl.seq0 + min(kj, len - 1);
   const char* kp = (const char*)((const T*)p.k + krow * p.k_row + pl.kvh * p.k_head);
   const char* vp = (const char*)((const T*)p.v + krow * p.v_row + pl.kvh * p.v_head);
 #pragma unroll
   for (int s = 0; s < G::NS; ++s) {
     kf[s] = *reinterpret_cast<const u32x4*>(kp + (2 * s + half) * 16);
-    vf[s] = *reinterpret_cast<const u32x4*>(vp + (2 * s + half) * 16);
-    if (kj >= len) kf[s] = vf[s] = u32x4{0, 0, 0, 0};
+    if (kj >= len) kf[s] = u32x4{0, 0, 0, 0};
+    if constexpr (!G::VLDS) {
+      vf[s] = *reinterpret_cast<const u32x4*>(vp + (2 * s + half) * 16);
+      if (kj >= len) vf[s] = u32x4{0, 0, 0, 0};
+    }
   }
-  keep(0);
+  keep(it0 & 1);
   const float c1 = p.scale * LOG2E;
   const int u0 = 4 * half + 127 - (w * 32 + m);
   const float* const bcopy = bv0 + (u0 & 3) * G::SEG;
@@ -721,25 +742,33 @@ __global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_ker
   float dacc[2 * NT + 1];
 #pragma unroll
   for (int j = 0; j <= 2 * NT; ++j) dacc[j] = 0.f;
-  float* const mine = strip0 + (w * 4 + (lane >> 4)) * (32 * NT) + (lane & 15) + 16 * (2 * NT - 1);
-  if (dbias) ring[tid] = 0.f;
+  constexpr int NDIAG = 132 + 16 * (2 * NT - 1);   // diagonals of a tile: 127 down to -4 - 16 (2 NT - 1)
+  float* const mine =
+      strip0 + ((w * 2 + ((lane >> 4) & 1)) * 2 + half) * (32 * NT) + (lane & 15) + 16 * (2 * NT - 1);
+  if (dbias && tid < RING) ring[tid] = 0.f;
 
-  // the strips of one tile into the ring; diagonal R is key - query relative to (kb0, qb)
+  // the strips of one tile into the ring; diagonal R is key - query relative to (kb0, qb). Strip
+  // (b = 2 w + kr, half) holds diagonals 16 b - 4 half + slot - 16 (2 NT - 1), so R meets 2 NT strips
+  // of each half
   auto fold = [&](int buf, int qb, int h, bool end) {
-    const int R = tid + 127 - (NDIAG - 1) + 16 * (3 - (2 * NT - 1));  // 127 down to -4 - 16 (2 NT - 1)
-    if (tid < NDIAG && R <= 127) {
+    const int R = tid + 128 - NDIAG;
+    if (tid < NDIAG) {
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int slot = R - 32 * (i >> 2) - 16 * (i & 1) + 4 * ((i >> 1) & 1) + 16 * (2 * NT - 1);
-        const bool in = (unsigned)slot < (unsigned)(32 * NT);
-        const float x = strip0[(buf * 16 + i) * (32 * NT) + (in ? slot : 0)];
-        s += in ? x : 0.f;
+      for (int hf = 0; hf < 2; ++hf) {
+        const int x = R + 4 * hf + 16 * (2 * NT - 1);
+#pragma unroll
+        for (int db = 0; db < 2 * NT; ++db) {
+          const int b = (x >> 4) - db;
+          const bool in = (unsigned)b < 8u;
+          const float y = strip0[((buf * 8 + (in ? b : 0)) * 2 + hf) * (32 * NT) + (x & 15) + 16 * db];
+          s += in ? y : 0.f;
+        }
       }
-      const int d = kb0 - qb + R;
-      s += ring[d & (RING - 1)];
+      float* const slot = ring + (unsigned)(kb0 - qb + R + (1 << 30)) % RING;
+      s += *slot;
       const bool done = end || R > 127 - KT;
-      ring[d & (RING - 1)] = done ? 0.f : s;
+      *slot = done ? 0.f : s;
       const int x = qb + 127 - R;
       const long long ld = slab_row(p.bias_len);
       if (done && x < min((int)ld, len + 127))
@@ -754,17 +783,17 @@ __global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_ker
     for (int j = 1; j <= 2 * NT; ++j) dacc[j] = 0.f;
   };
 
-  int g = 0, qt = qt0;
-  const int total = group * nq;
   const bool part_block = kb0 + BQ > len;
-  auto tile = [&](const int it, auto masked_c) {
-    constexpr bool MASKED = decltype(masked_c)::value;
+  for (int it = it0; it < it1; ++it) {
+    // (one body and a branch around the masking alone: two bodies in the loop made the compiler copy
+    // the accumulators between them)
+    const bool masked = part_block || (CAUSAL && qt * KT < kb0 + BQ - 1);
     const int buf = it & 1, qb = qt * KT;
     char* const Qt = dyn + buf * 2 * G::TILE;
     char* const Ot = Qt + G::TILE;
     const float* const rb = rows0 + buf * 3 * KT + 4 * half;
     wait_all_and_meet();
-    if (it + 1 < total) {
+    if (it + 1 < it1) {
       const bool next_head = qt + 1 == qtn;
       fetch(h0 + g + next_head, next_head ? qt0 : qt + 1, buf ^ 1);
     }
@@ -775,59 +804,82 @@ __global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_ker
         f32x16 s, dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < G::NS; ++c) {
           mma_row<T>(L.rd_row(Qt, t, c), kf[c], s);
-          mma_row<T>(L.rd_row(Ot, t, c), vf[c], dp);
+          mma_row<T>(L.rd_row(Ot, t, c), G::VLDS ? L.rd_row(vt, 0, c) : vf[G::VLDS ? 0 : c], dp);
         }
-        float pr[16], ds[16];
+        {
+          constexpr int RD = G::VLDS ? 3 : 2, MM = sizeof(T) == 2 ? 2 : 8;
+          __builtin_amdgcn_sched_group_barrier(0x100, RD, 0);
+#pragma unroll
+          for (int c = 0; c + 1 < G::NS; ++c) {
+            __builtin_amdgcn_sched_group_barrier(0x100, RD, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, MM, 0);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x8, MM, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float pr[16];
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           const float4 l4 = *reinterpret_cast<const float4*>(rb + 32 * t + 8 * a);
-          const float4 d4 = *reinterpret_cast<const float4*>(rb + KT + 32 * t + 8 * a);
-          const float l[4] = {l4.x, l4.y, l4.z, l4.w}, d[4] = {d4.x, d4.y, d4.z, d4.w};
-          float gg[4], b[4];
+          const float l[4] = {l4.x, l4.y, l4.z, l4.w};
           if constexpr (BIAS) {
             const float4 g4 = *reinterpret_cast<const float4*>(rb + 2 * KT + 32 * t + 8 * a);
             const float4 b4 = *reinterpret_cast<const float4*>(bcopy + buf * 4 * G::SEG + bv_pos(uj + 32 * t + 8 * a, us));
-            gg[0] = g4.x; gg[1] = g4.y; gg[2] = g4.z; gg[3] = g4.w;
-            b[0] = b4.x; b[1] = b4.y; b[2] = b4.z; b[3] = b4.w;
+            pr[4 * a] = fmaf(s[4 * a], c1, fmaf(g4.x * LOG2E, b4.x, -l[0]));
+            pr[4 * a + 1] = fmaf(s[4 * a + 1], c1, fmaf(g4.y * LOG2E, b4.y, -l[1]));
+            pr[4 * a + 2] = fmaf(s[4 * a + 2], c1, fmaf(g4.z * LOG2E, b4.z, -l[2]));
+            pr[4 * a + 3] = fmaf(s[4 * a + 3], c1, fmaf(g4.w * LOG2E, b4.w, -l[3]));
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) pr[4 * a + c] = fmaf(s[4 * a + c], c1, -l[c]);
           }
+        }
+        if (masked) {
+          asm volatile("");
+          const int first = CAUSAL ? (kj < len ? kj : 1 << 30) : (kj < len ? 0 : 1 << 30);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            pr[r] = qb + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) >= first ? pr[r] : -INF;
+        }
+        float ds[16];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const float4 d4 = *reinterpret_cast<const float4*>(rb + KT + 32 * t + 8 * a);
+          const float d[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int r = 4 * a + c;
-            float e = fmaf(s[r], c1, BIAS ? fmaf(gg[c] * LOG2E, b[c], -l[c]) : -l[c]);
-            if constexpr (MASKED) {
-              const int qi = qb + 32 * t + 8 * a + 4 * half + c;
-              e = (kj < len && (!CAUSAL || kj <= qi)) ? e : -INF;
-            }
-            pr[r] = exp2_(e);
-            ds[r] = pr[r] * (dp[r] - d[c]);
+            pr[4 * a + c] = exp2_(pr[4 * a + c]);
+            ds[4 * a + c] = pr[4 * a + c] * (dp[4 * a + c] - d[c]);
           }
           if constexpr (BIAS) {
             // (a, c): shift 8 (a & 1) + c, accumulator 2 t + (a >> 1)
+            const float4 gg = *reinterpret_cast<const float4*>(rb + 2 * KT + 32 * t + 8 * a);
             float& lo = dacc[2 * t + (a >> 1)];
             float& hi = dacc[2 * t + (a >> 1) + 1];
             if (a & 1) {
-              diag_add<8>(gg[0] * ds[4 * a], lo, hi);
-              diag_add<9>(gg[1] * ds[4 * a + 1], lo, hi);
-              diag_add<10>(gg[2] * ds[4 * a + 2], lo, hi);
-              diag_add<11>(gg[3] * ds[4 * a + 3], lo, hi);
+              diag_add<8>(gg.x * ds[4 * a], lo, hi);
+              diag_add<9>(gg.y * ds[4 * a + 1], lo, hi);
+              diag_add<10>(gg.z * ds[4 * a + 2], lo, hi);
+              diag_add<11>(gg.w * ds[4 * a + 3], lo, hi);
             } else {
-              diag_add<0>(gg[0] * ds[4 * a], lo, hi);
-              diag_add<1>(gg[1] * ds[4 * a + 1], lo, hi);
-              diag_add<2>(gg[2] * ds[4 * a + 2], lo, hi);
-              diag_add<3>(gg[3] * ds[4 * a + 3], lo, hi);
+              diag_add<0>(gg.x * ds[4 * a], lo, hi);
+              diag_add<1>(gg.y * ds[4 * a + 1], lo, hi);
+              diag_add<2>(gg.z * ds[4 * a + 2], lo, hi);
+              diag_add<3>(gg.w * ds[4 * a + 3], lo, hi);
             }
           }
         }
-        mma_col<T, D>(L, Ot, 32 * t, pr, dv, lane);
-        mma_col<T, D>(L, Qt, 32 * t, ds, dk, lane);
+        mma_col<T, G>(L, Ot, 32 * t, pr, dv, lane);
+        mma_col<T, G>(L, Qt, 32 * t, ds, dk, lane);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (dbias) shed(buf);
-    if (it + 1 < total) keep(buf ^ 1);
+    if (it + 1 < it1) keep(buf ^ 1);
     if (dbias && qt + 1 == qtn) {
       // the head's last tile: fold it and the accumulators' rest, and empty the ring
       __syncthreads();
@@ -839,16 +891,24 @@ __global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_ker
 #pragma unroll
       for (int j = 0; j <= 2 * NT; ++j) dacc[j] = 0.f;
     }
-  };
-  for (int it = 0; it < total; ++it) {
-    if (part_block || (CAUSAL && qt * KT < kb0 + BQ - 1)) tile(it, std::true_type{});
-    else tile(it, std::false_type{});
     if (++qt == qtn) {
       qt = qt0;
       ++g;
     }
   }
   if (kj >= len) return;
+  if (sums) {   // this slice's f32 sums; dkv_kernel adds the slices in order
+    const long long n = p.rows * p.hkv * D;
+    float* const a = sums + pl.g * 2 * n + (krow * p.hkv + pl.kvh) * D + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        store4<float>(a + 32 * dt + 8 * i, dk[dt][4 * i], dk[dt][4 * i + 1], dk[dt][4 * i + 2], dk[dt][4 * i + 3]);
+        store4<float>(a + n + 32 * dt + 8 * i, dv[dt][4 * i], dv[dt][4 * i + 1], dv[dt][4 * i + 2], dv[dt][4 * i + 3]);
+      }
+    return;
+  }
   T* const dko = (T*)p.dk + krow * p.dk_row + pl.kvh * p.dk_head + 4 * half;
   T* const dvo = (T*)p.dv + krow * p.dv_row + pl.kvh * p.dv_head + 4 * half;
 #pragma unroll
@@ -859,6 +919,32 @@ __global__ __launch_bounds__(256, (D * sizeof(T) > 128 ? 1 : 2)) void bwd_kv_ker
                 dk[dt][4 * a + 3] * p.scale);
       store4<T>(dvo + 32 * dt + 8 * a, dv[dt][4 * a], dv[dt][4 * a + 1], dv[dt][4 * a + 2], dv[dt][4 * a + 3]);
     }
+}
+
+// dk, dv = the slices' f32 sums, added in order: one workgroup per block of rows and key head
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dkv_kernel(const nrse_attn_packed_bwd_params p, int slices,
+                                                  const float* __restrict__ sums) {
+  const int nblk = (int)(p.rows / BQ) + p.nseq;
+  const Place pl = place(nblk, p.hkv, 1);
+  if (pl.block >= nblk) return;
+  const Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
+  if (!bl.any) return;
+  const int n4 = min(BQ, bl.len - bl.row0) * (D / 4);
+  const long long n = p.rows * p.hkv * D;
+  for (int i = threadIdx.x; i < n4; i += 256) {
+    const long long row = bl.seq0 + bl.row0 + i / (D / 4);
+    const int d = i % (D / 4) * 4;
+    const float* a = sums + (row * p.hkv + pl.kvh) * D + d;
+    float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+    for (int s = 0; s < slices; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(a + s * 2 * n), y = *reinterpret_cast<const float4*>(a + s * 2 * n + n);
+      k.x += x.x; k.y += x.y; k.z += x.z; k.w += x.w;
+      v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+    }
+    store4<T>((T*)p.dk + row * p.dk_row + pl.kvh * p.dk_head + d, k.x * p.scale, k.y * p.scale, k.z * p.scale, k.w * p.scale);
+    store4<T>((T*)p.dv + row * p.dv_row + pl.kvh * p.dv_head + d, v.x, v.y, v.z, v.w);
+  }
 }
 
 // dbias[h, d] (+)= the slab's rows: for each diagonal, the blocks that hold it, in block order within 4
@@ -942,9 +1028,23 @@ template <typename T, int D>
 size_t lds_fwd(bool bias) { return 4 * Geo<T, D>::TILE + (bias ? 8 * Geo<T, D>::SEG * sizeof(float) : 0); }
 template <typename T, int D>
 size_t lds_kv(bool bias) {
-  using G = Geo<T, D>;
-  return 4 * G::TILE + 6 * G::KT * sizeof(float) +
+  using G = KvGeo<T, D>;
+  return (G::VLDS ? 8 : 4) * G::TILE + 6 * G::KT * sizeof(float) +
          (bias ? (8 * G::SEG + 2 * 16 * 32 * G::NT + RING) * sizeof(float) : 0);
+}
+
+// Slices of a key block's (head, query tile) pairs: a chip of 256 CUs takes 512 of these workgroups at
+// once, and a batch with fewer blocks x key heads is split up to 8 ways, each slice writing f32 sums that
+// dkv_kernel adds. Not below 8 pairs a slice (of an average sequence); whole heads where a bias
+// gradient is summed.
+int kv_slices(const nrse_attn_packed_bwd_params& p) {
+  const long long groups = (p.rows / BQ + p.nseq) * p.hkv, G = p.hq / p.hkv;
+  const long long kt = p.head_dim * (p.dtype == NRSE_BF16 ? 2 : 4) > 128 ? 32 : 64;
+  long long n = (512 + groups - 1) / groups;
+  n = std::min(n, std::min(8LL, std::max(1LL, G * (p.rows / p.nseq) / kt / 8)));
+  if (p.bias_vec)
+    while (G % n) --n;
+  return (int)n;
 }
 
 template <typename T, int D, bool BIAS, bool CAUSAL>
@@ -952,13 +1052,23 @@ void launch_fwd(const nrse_attn_packed_fwd_params& p, hipStream_t st) {
   const long long n = grid_size(p.rows / BQ + p.nseq, p.hkv, p.hq / p.hkv);
   hipLaunchKernelGGL((fwd_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)n), dim3(256), (lds_fwd<T, D>(BIAS)), st, p);
 }
+// the workspace: the bias gradient's table of blocks and slab, then the slices' sums
+long long slab_floats(const nrse_attn_packed_bwd_params& p) {
+  const long long nblk = p.rows / BQ + p.nseq;
+  return p.bias_vec && p.dbias_vec ? nblk * 4 + p.hq * nblk * slab_row(p.bias_len) : 0;
+}
+
 template <typename T, int D, bool BIAS, bool CAUSAL>
 void launch_bwd(const nrse_attn_packed_bwd_params& p, hipStream_t st) {
   const long long nblk = p.rows / BQ + p.nseq;
   hipLaunchKernelGGL((bwd_q_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, p.hq / p.hkv)), dim3(256),
                      (lds_fwd<T, D>(BIAS)), st, p);
-  hipLaunchKernelGGL((bwd_kv_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, 1)), dim3(256),
-                     (lds_kv<T, D>(BIAS)), st, p);
+  const int ns = kv_slices(p);
+  float* const sums = ns > 1 ? p.part + slab_floats(p) : nullptr;
+  hipLaunchKernelGGL((bwd_kv_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, ns)), dim3(256),
+                     (lds_kv<T, D>(BIAS)), st, p, ns, sums);
+  if (ns > 1)
+    hipLaunchKernelGGL((dkv_kernel<T, D>), dim3((unsigned)grid_size(nblk, p.hkv, 1)), dim3(256), 0, st, p, ns, sums);
 }
 
 template <typename P, typename F>
@@ -1028,9 +1138,9 @@ extern "C" int nrse_attn_packed_fwd(const nrse_attn_packed_fwd_params* p, void* 
 extern "C" long long nrse_attn_packed_bwd_workspace(const nrse_attn_packed_bwd_params* p) {
   NRSE_CHECK_PARAMS(p, "nrse_attn_packed_bwd_workspace");
   if (const int rc = check_common("nrse_attn_packed_bwd_workspace", p)) return rc;
-  if (!p->bias_vec || !p->dbias_vec) return 0;
-  const long long nblk = p->rows / BQ + p->nseq;
-  return nblk * 4 + p->hq * nblk * slab_row(p->bias_len);
+  if (p->rows == 0 || p->nseq == 0) return 0;
+  const int ns = kv_slices(*p);
+  return slab_floats(*p) + (ns > 1 ? 2LL * ns * p->rows * p->hkv * p->head_dim : 0);
 }
 
 extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* stream) {
@@ -1056,7 +1166,7 @@ extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* 
   ROWS_KV(fn, dk);
   ROWS_KV(fn, dv);
   NRSE_REQUIRE(p->lse && p->delta, "%s: lse and delta are needed", fn);
-  NRSE_REQUIRE(!p->dbias_vec || p->part, "%s: dbias_vec needs the workspace (nrse_attn_packed_bwd_workspace)", fn);
+  NRSE_REQUIRE(p->part || nrse_attn_packed_bwd_workspace(p) == 0, "%s: part, the workspace, is null", fn);
   dispatch(*p, [&](auto t, auto d, auto b, auto c) {
     launch_bwd<decltype(t), decltype(d)::value, decltype(b)::value, decltype(c)::value>(*p, st);
   });

@@ -61,7 +61,7 @@ def test_refusals(kw, word):
     (dict(dv=None), "dv is null"), (dict(lse=None), "lse"), (dict(delta=None), "delta"),
     (dict(dbias_vec=A), "not there"), (dict(dgate=A), "not there"),
     (dict(bias_vec=A, bias_len=300, dgate=A), "without a gate"),
-    (dict(bias_vec=A, bias_len=300, dbias_vec=A), "workspace")])
+    (dict(bias_vec=A, bias_len=300, dbias_vec=A), "workspace"), (dict(rows=4096, nseq=1), "workspace")])
 def test_backward_refusals(kw, word):
     L = _lib.lib()
     assert L.nrse_attn_packed_bwd(ctypes.byref(bwd_params(**kw)), None) < 0
@@ -88,11 +88,19 @@ def test_nothing_to_do_is_no_error():
         assert L.nrse_attn_packed_bwd(ctypes.byref(bwd_params(**kw)), None) == 0
 
 
-def test_workspace_only_for_the_bias_gradient():
+def test_workspace():
+    """The bias gradient's slab, and the sums of sliced key blocks where a batch has too few of them for the chip; a
+    batch with enough blocks needs neither."""
     L = _lib.lib()
-    assert L.nrse_attn_packed_bwd_workspace(ctypes.byref(bwd_params())) == 0
-    assert L.nrse_attn_packed_bwd_workspace(ctypes.byref(bwd_params(bias_vec=A, bias_len=256))) == 0
-    assert L.nrse_attn_packed_bwd_workspace(ctypes.byref(bwd_params(bias_vec=A, bias_len=256, dbias_vec=A))) > 0
+
+    def floats(**kw):
+        return L.nrse_attn_packed_bwd_workspace(ctypes.byref(bwd_params(**kw)))
+    assert floats(rows=100000, hkv=8, nseq=10) == 0
+    assert floats(rows=100000, hkv=8, nseq=10, bias_vec=A, bias_len=256) == 0
+    assert floats(rows=100000, hkv=8, nseq=10, bias_vec=A, bias_len=256, dbias_vec=A) > 0
+    few = floats(rows=4096, hkv=1, nseq=1)
+    assert few > 0 and few % (2 * 4096 * 64) == 0
+    assert floats(rows=0) == 0 and floats(nseq=0) == 0
 
 
 def test_wrappers_take_device_tensors_only():
