@@ -25,7 +25,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short short8v __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void_t;
 
-constexpr int BQ = 128;       // rows of a workgroup
+constexpr int BQ = 128;       // keys of a dK/dV workgroup, rows of a forward or dQ one of one stream
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float INF = __builtin_huge_valf();
@@ -35,8 +35,9 @@ constexpr float RESCALE_TAU = 8.f;
 
 NRSE_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-constexpr int tile_rows(int row_bytes) { return row_bytes > 256 ? 32 : 64; }
-template <typename T, int D, int KT_ = tile_rows(D * (int)sizeof(T))>
+// rows of a streamed tile, for ST streams: what keeps two workgroups on a CU (one at 512-byte rows)
+constexpr int tile_rows(int row_bytes, int ST) { return ST == 1 ? (row_bytes > 256 ? 32 : 64) : ST == 2 && row_bytes == 128 ? 64 : 32; }
+template <typename T, int D, int KT_>
 struct Geo {
   static constexpr int RB = D * (int)sizeof(T);         // bytes of a row
   static constexpr int PANELS = RB / 128;               // a tile is kept in panels of 128-byte rows
@@ -47,6 +48,21 @@ struct Geo {
   static constexpr int NT = KT / 32;                    // 32-row pieces of a tile
   static constexpr int DMA = KT / 8 * PANELS / 4;       // LDS-DMA instructions per wave and tile
   static constexpr int SEG = 192;                       // bias entries of a workgroup's tile, KT + 127, in 64s
+};
+
+// The forward and dQ kernels in ST streams: the 4 waves are 4 / ST pieces of 32 rows times ST streams,
+// and stream i takes every ST-th key tile, its running maximum, sum and output joined with the others' in
+// LDS at the end. A workgroup then has 128 / ST rows: more of them, each ST times shorter.
+template <typename T, int D, int ST>
+struct QGeo : Geo<T, D, tile_rows(D * (int)sizeof(T), ST)> {
+  using B = Geo<T, D, tile_rows(D * (int)sizeof(T), ST)>;
+  static constexpr int BR = 128 / ST;                               // rows of a workgroup
+  static constexpr int SEG = ST == 1 ? 192 : ST == 2 ? 128 : 64;    // >= KT + BR - 1, in 64s
+  static_assert(SEG >= B::KT + BR - 1 && SEG * ST <= 256, "a bias entry per thread");
+  static constexpr int BUF = 2 * B::TILE;                           // K and V tile
+  static constexpr int KV_LDS = ST * 2 * BUF;                       // [ST][2 buffers]
+  static constexpr int WAVES = ST == 1 && B::RB == 128 ? 3 : 2;     // of the forward per SIMD
+  static constexpr int Q_WAVES = B::RB > 256 ? 1 : 2;               // of dQ
 };
 
 // ---------------------------------------------------------------------------------- LDS tiles
@@ -177,10 +193,11 @@ struct Dma {
 // ---------------------------------------------------------------------------------- which rows
 // The blocks of all sequences are numbered from the last sequence's last block down: under a causal
 // mask a block's work grows with its place, so the long ones of a sequence go first. The grid is
-// sized from what the host knows, rows / BQ + sequences, and what is left over ends at once.
+// sized from what the host knows, rows / BR + sequences, and what is left over ends at once.
 // Bounds are taken from cu_seqlens as they stand in device memory, clamped to the tensors.
 struct Block { int seq0, len, row0; bool any; };
 
+template <int BR>
 NRSE_DEV Block find_block(const int* __restrict__ cu, const int* __restrict__ used, int nseq, int rows, int want) {
   const int lane = threadIdx.x & 63;
   int before = 0;
@@ -192,7 +209,7 @@ NRSE_DEV Block find_block(const int* __restrict__ cu, const int* __restrict__ us
       len = min(max(cu[s + 1], start), rows) - start;
       if (used) len = min(len, max(used[s], 0));
     }
-    const int nb = (len + BQ - 1) / BQ;
+    const int nb = (len + BR - 1) / BR;
     int incl = nb;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -205,7 +222,7 @@ NRSE_DEV Block find_block(const int* __restrict__ cu, const int* __restrict__ us
       const int first = before + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(nb, l);
       const int n = __builtin_amdgcn_readlane(nb, l);
       return Block{__builtin_amdgcn_readlane(start, l), __builtin_amdgcn_readlane(len, l),
-                   (n - 1 - (want - first)) * BQ, true};
+                   (n - 1 - (want - first)) * BR, true};
     }
     before += __builtin_amdgcn_readlane(incl, 63);
   }
@@ -266,17 +283,17 @@ NRSE_DEV void wait_all_and_meet() {
 }
 
 // ---------------------------------------------------------------------------------- forward
-template <typename T, int D, bool BIAS, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_params p) {
-  using G = Geo<T, D>;
+template <typename T, int D, bool BIAS, bool CAUSAL, int ST>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::WAVES, QGeo<T, D, ST>::WAVES))) void fwd_kernel(const nrse_attn_packed_fwd_params p) {
+  using G = QGeo<T, D, ST>;
   constexpr int KT = G::KT;
   extern __shared__ __attribute__((aligned(16))) char dyn[];
-  float* const bv0 = reinterpret_cast<float*>(dyn + 4 * G::TILE);  // [2][4][SEG]
+  float* const bv0 = reinterpret_cast<float*>(dyn + G::KV_LDS);  // [ST][2][4][SEG]
   const int group = p.hq / p.hkv;
-  const int nblk = (int)(p.rows / BQ) + p.nseq;
+  const int nblk = (int)(p.rows / G::BR) + p.nseq;
   const Place pl = place(nblk, p.hkv, group);
   if (pl.block >= nblk) return;
-  const Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
+  const Block bl = find_block<G::BR>(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
   if (!bl.any) return;
   const int h = pl.kvh * group + pl.g, len = bl.len;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -284,22 +301,32 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_
   const int m = lane & 31, half = lane >> 5;
   Lds<T, G> L;
   L.init(lane);
-  const int q0 = bl.row0 + w * 32;       // this wave's first row in the sequence
+  const int st = w / (4 / ST), sub = w % (4 / ST);
+  const int q0 = bl.row0 + sub * 32;     // this wave's first row in the sequence
   const int qi = q0 + m;
   const bool live = q0 < len;            // a wave past the end keeps its share of the copies and the barriers
   Dma<T, G> kd, vd;
   kd.init((const T*)p.k + (long long)bl.seq0 * p.k_row + pl.kvh * p.k_head, p.k_row, len, lane);
   vd.init((const T*)p.v + (long long)bl.seq0 * p.v_row + pl.kvh * p.v_head, p.v_row, len, lane);
-  const int kend = CAUSAL ? min(len, bl.row0 + BQ) : len;
-  const int ntiles = (kend + KT - 1) / KT;
-  kd.issue(dyn, 0, w);
-  vd.issue(dyn + G::TILE, 0, w);
+  const int kend = CAUSAL ? min(len, bl.row0 + G::BR) : len;
+  const int ntiles = (kend + KT - 1) / KT, nit = (ntiles + ST - 1) / ST;
+  auto issue = [&](int it) {   // start bringing every stream's tile of iteration `it`
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+      char* const K = dyn + (i * 2 + (it & 1)) * G::BUF;
+      kd.issue(K, (it * ST + i) * KT, w);
+      vd.issue(K + G::TILE, (it * ST + i) * KT, w);
+    }
+  };
+  issue(0);
   const int nd = 2 * p.bias_len - 1;
   const float* vec = BIAS ? p.bias_vec + (long long)h * nd : nullptr;
-  // segment entry j of the tile at key kb: b[kb - row0 + j - 127]
-  const int e0 = p.bias_len - 1 - bl.row0 - 127;
+  // segment entry j of the tile at key kb: b[kb - row0 + j - (BR - 1)]; a thread brings one entry of its
+  // stream's segment
+  const int bst = ST == 1 ? 0 : tid / G::SEG, bt = ST == 1 ? tid : tid % G::SEG;
+  const int e0 = p.bias_len - 1 - bl.row0 - (G::BR - 1) + bst * KT + bt;
   float bnext = 0.f;
-  if constexpr (BIAS) bv_store<G::SEG>(bv0, tid, bv_load(vec, nd, e0 + tid));
+  if constexpr (BIAS) bv_store<G::SEG>(bv0 + bst * 8 * G::SEG, bt, bv_load(vec, nd, e0));
   u32x4 qf[G::NS];
   const int qc = min(qi, len - 1);       // loads from a row that is there, zeroed after
   const T* qrow = (const T*)p.q + (long long)(bl.seq0 + qc) * p.q_row + h * p.q_head;
@@ -313,8 +340,8 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_
   if constexpr (BIAS) {
     if (p.gate) gl = p.gate[h * p.rows + bl.seq0 + qc] * LOG2E;
   }
-  const int u0 = 4 * half + 127 - (w * 32 + m);
-  const float* const bcopy = bv0 + (u0 & 3) * G::SEG;
+  const int u0 = 4 * half + G::BR - 1 - (sub * 32 + m);
+  const float* const bcopy = bv0 + st * 8 * G::SEG + (u0 & 3) * G::SEG;
   const int uj = u0 - (u0 & 3), us = u0 & 3;
 
   float mref = 0.f, thr = -INF, lsum = 0.f;
@@ -326,8 +353,8 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_
 
   auto tile = [&](const int it, auto masked_c) {
     constexpr bool MASKED = decltype(masked_c)::value;
-    const int kb = it * KT;
-    char* const Kt = dyn + (it & 1) * 2 * G::TILE;
+    const int kb = (it * ST + st) * KT;
+    char* const Kt = dyn + (st * 2 + (it & 1)) * G::BUF;
     char* const Vt = Kt + G::TILE;
     wait_all_and_meet();
     float4 bb[G::NT][4];
@@ -340,21 +367,36 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_
         for (int a = 0; a < 4; ++a)
           bb[t][a] = *reinterpret_cast<const float4*>(bcopy + (it & 1) * 4 * G::SEG + bv_pos(uj + 32 * t + 8 * a, us));
     }
-    if (it + 1 < ntiles) {
-      char* const Kn = dyn + ((it + 1) & 1) * 2 * G::TILE;
-      kd.issue(Kn, kb + KT, w);
-      vd.issue(Kn + G::TILE, kb + KT, w);
-      if constexpr (BIAS) bnext = bv_load(vec, nd, e0 + kb + KT + tid);
+    if (it + 1 < nit) {
+      issue(it + 1);
+      if constexpr (BIAS) bnext = bv_load(vec, nd, e0 + (it + 1) * ST * KT);
     }
-    if (live && (!CAUSAL || kb <= q0 + 31)) {
+    if (live && (ST == 1 || kb < kend) && (!CAUSAL || kb <= q0 + 31)) {
       float v[G::NT][16];
+      f32x16 sv[G::NT];
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < G::NT; ++t) {
-        f32x16 s;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        for (int r = 0; r < 16; ++r) sv[t][r] = 0.f;
 #pragma unroll
-        for (int c = 0; c < G::NS; ++c) mma_row<T>(L.rd_row(Kt, t, c), qf[c], s);
+        for (int c = 0; c < G::NS; ++c) mma_row<T>(L.rd_row(Kt, t, c), qf[c], sv[t]);
+      }
+      if constexpr (sizeof(T) == 2) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < G::NS * G::NT - 4; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < G::NT; ++t) {
+        const f32x16& s = sv[t];
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           if constexpr (BIAS) {
@@ -414,15 +456,54 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_
       }
     }
     if constexpr (BIAS) {
-      if (it + 1 < ntiles) bv_store<G::SEG>(bv0 + ((it + 1) & 1) * 4 * G::SEG, tid, bnext);
+      if (it + 1 < nit) bv_store<G::SEG>(bv0 + (bst * 2 + ((it + 1) & 1)) * 4 * G::SEG, bt, bnext);
     }
   };
   // tiles that every row of the workgroup sees whole, then those with a mask
-  const int nfull = min(len, CAUSAL ? bl.row0 + 1 : len) / KT;
+  const int nfull = min(len, CAUSAL ? bl.row0 + 1 : len) / (KT * ST);
   for (int it = 0; it < nfull; ++it) tile(it, std::false_type{});
-  for (int it = nfull; it < ntiles; ++it) tile(it, std::true_type{});
+  for (int it = nfull; it < nit; ++it) tile(it, std::true_type{});
 
-  const float l = xor32_sum(lsum);
+  float l = xor32_sum(lsum);
+  if constexpr (ST > 1) {
+    // join: out = sum 2^(m_i - M) o_i over the streams, in stream order
+    float* const js = reinterpret_cast<float*>(dyn);
+    constexpr int PER = (D / 2 + 2) * 64;   // a wave's accumulators, maximum and sum
+    float* const at = js + ((st - 1) * (4 / ST) + sub) * PER + lane;
+    const float mine = thr < 0.f ? -INF : mref;
+    __syncthreads();
+    if (st > 0) {
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) at[(dt * 16 + r) * 64] = o[dt][r];
+      at[(D / 2) * 64] = mine;
+      at[(D / 2 + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (st > 0) return;
+    const float* from = js + sub * PER + lane;
+    float M = mine;
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) M = fmaxf(M, from[i * (4 / ST) * PER + (D / 2) * 64]);
+    const float a0 = M > -INF ? exp2_(mine - M) : 0.f;
+    l *= a0;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] *= a0;
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) {
+      const float* const x = from + i * (4 / ST) * PER;
+      const float a = M > -INF ? exp2_(x[(D / 2) * 64] - M) : 0.f;
+      l = fmaf(a, x[(D / 2 + 1) * 64], l);
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] = fmaf(a, x[(dt * 16 + r) * 64], o[dt][r]);
+    }
+    mref = M > -INF ? M : 0.f;
+  }
   if (qi >= len) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a row whose bias leaves nothing: zeros
   T* const orow = (T*)p.out + (long long)(bl.seq0 + qi) * p.out_row + h * p.out_head + 4 * half;
@@ -441,17 +522,17 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(const nrse_attn_packed_fwd_
 // Without a bias delta is rowsum(dO O), from the stored output. The gradients of bias and gate are f32
 // outputs, and the rounding of a bf16 O would be all their error: there delta is summed again as
 // sum_j P dP from the f32 accumulators, and dgate = sum P dP b - delta sum P b.
-template <typename T, int D, bool BIAS, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bwd_params p) {
-  using G = Geo<T, D>;
+template <typename T, int D, bool BIAS, bool CAUSAL, int ST>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::Q_WAVES, QGeo<T, D, ST>::Q_WAVES))) void bwd_q_kernel(const nrse_attn_packed_bwd_params p) {
+  using G = QGeo<T, D, ST>;
   constexpr int KT = G::KT;
   extern __shared__ __attribute__((aligned(16))) char dyn[];
-  float* const bv0 = reinterpret_cast<float*>(dyn + 4 * G::TILE);
+  float* const bv0 = reinterpret_cast<float*>(dyn + G::KV_LDS);
   const int group = p.hq / p.hkv;
-  const int nblk = (int)(p.rows / BQ) + p.nseq;
+  const int nblk = (int)(p.rows / G::BR) + p.nseq;
   const Place pl = place(nblk, p.hkv, group);
   if (pl.block >= nblk) return;
-  const Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
+  const Block bl = find_block<G::BR>(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
   if (!bl.any) return;
   const int h = pl.kvh * group + pl.g, len = bl.len;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -459,22 +540,31 @@ __global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bw
   const int m = lane & 31, half = lane >> 5;
   Lds<T, G> L;
   L.init(lane);
-  const int q0 = bl.row0 + w * 32;
+  const int st = w / (4 / ST), sub = w % (4 / ST);
+  const int q0 = bl.row0 + sub * 32;
   const int qi = q0 + m;
   const bool live = q0 < len;
   Dma<T, G> kd, vd;
   kd.init((const T*)p.k + (long long)bl.seq0 * p.k_row + pl.kvh * p.k_head, p.k_row, len, lane);
   vd.init((const T*)p.v + (long long)bl.seq0 * p.v_row + pl.kvh * p.v_head, p.v_row, len, lane);
-  const int kend = CAUSAL ? min(len, bl.row0 + BQ) : len;
-  const int ntiles = (kend + KT - 1) / KT;
-  kd.issue(dyn, 0, w);
-  vd.issue(dyn + G::TILE, 0, w);
+  const int kend = CAUSAL ? min(len, bl.row0 + G::BR) : len;
+  const int ntiles = (kend + KT - 1) / KT, nit = (ntiles + ST - 1) / ST;
+  auto issue = [&](int it) {   // start bringing every stream's tile of iteration `it`
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+      char* const K = dyn + (i * 2 + (it & 1)) * G::BUF;
+      kd.issue(K, (it * ST + i) * KT, w);
+      vd.issue(K + G::TILE, (it * ST + i) * KT, w);
+    }
+  };
+  issue(0);
   const int nd = 2 * p.bias_len - 1;
   const float* vec = BIAS ? p.bias_vec + (long long)h * nd : nullptr;
-  const int e0 = p.bias_len - 1 - bl.row0 - 127;
+  const int bst = ST == 1 ? 0 : tid / G::SEG, bt = ST == 1 ? tid : tid % G::SEG;
+  const int e0 = p.bias_len - 1 - bl.row0 - (G::BR - 1) + bst * KT + bt;
   float bnext = 0.f;
   // (kept finite: P = 0 where the bias is -inf, and 0 * -inf would reach dgate)
-  if constexpr (BIAS) bv_store<G::SEG>(bv0, tid, fmaxf(bv_load(vec, nd, e0 + tid), -3e38f));
+  if constexpr (BIAS) bv_store<G::SEG>(bv0 + bst * 8 * G::SEG, bt, fmaxf(bv_load(vec, nd, e0), -3e38f));
   u32x4 qf[G::NS], df[G::NS];
   const int qc = min(qi, len - 1);
   const long long row = bl.seq0 + qc;
@@ -506,8 +596,8 @@ __global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bw
   }
   float lse2 = p.lse[h * p.rows + row] * LOG2E;
   if (lse2 == -INF) lse2 = INF;  // nothing left in this row: P = 0
-  const int u0 = 4 * half + 127 - (w * 32 + m);
-  const float* const bcopy = bv0 + (u0 & 3) * G::SEG;
+  const int u0 = 4 * half + G::BR - 1 - (sub * 32 + m);
+  const float* const bcopy = bv0 + st * 8 * G::SEG + (u0 & 3) * G::SEG;
   const int uj = u0 - (u0 & 3), us = u0 & 3;
   float sum_pd = 0.f, sum_pb = 0.f, sum_pdb = 0.f;
   f32x16 dq[G::DT];
@@ -518,8 +608,8 @@ __global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bw
 
   auto tile = [&](const int it, auto masked_c) {
     constexpr bool MASKED = decltype(masked_c)::value;
-    const int kb = it * KT;
-    char* const Kt = dyn + (it & 1) * 2 * G::TILE;
+    const int kb = (it * ST + st) * KT;
+    char* const Kt = dyn + (st * 2 + (it & 1)) * G::BUF;
     char* const Vt = Kt + G::TILE;
     wait_all_and_meet();
     float4 bb[G::NT][4];
@@ -530,13 +620,11 @@ __global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bw
         for (int a = 0; a < 4; ++a)
           bb[t][a] = *reinterpret_cast<const float4*>(bcopy + (it & 1) * 4 * G::SEG + bv_pos(uj + 32 * t + 8 * a, us));
     }
-    if (it + 1 < ntiles) {
-      char* const Kn = dyn + ((it + 1) & 1) * 2 * G::TILE;
-      kd.issue(Kn, kb + KT, w);
-      vd.issue(Kn + G::TILE, kb + KT, w);
-      if constexpr (BIAS) bnext = fmaxf(bv_load(vec, nd, e0 + kb + KT + tid), -3e38f);
+    if (it + 1 < nit) {
+      issue(it + 1);
+      if constexpr (BIAS) bnext = fmaxf(bv_load(vec, nd, e0 + (it + 1) * ST * KT), -3e38f);
     }
-    if (live && (!CAUSAL || kb <= q0 + 31)) {
+    if (live && (ST == 1 || kb < kend) && (!CAUSAL || kb <= q0 + 31)) {
       const int last = CAUSAL ? min(len - 1, qi) : len - 1;
 #pragma unroll
       for (int t = 0; t < G::NT; ++t) {
@@ -571,13 +659,45 @@ __global__ __launch_bounds__(256, 2) void bwd_q_kernel(const nrse_attn_packed_bw
       }
     }
     if constexpr (BIAS) {
-      if (it + 1 < ntiles) bv_store<G::SEG>(bv0 + ((it + 1) & 1) * 4 * G::SEG, tid, bnext);
+      if (it + 1 < nit) bv_store<G::SEG>(bv0 + (bst * 2 + ((it + 1) & 1)) * 4 * G::SEG, bt, bnext);
     }
   };
-  const int nfull = min(len, CAUSAL ? bl.row0 + 1 : len) / KT;
+  const int nfull = min(len, CAUSAL ? bl.row0 + 1 : len) / (KT * ST);
   for (int it = 0; it < nfull; ++it) tile(it, std::false_type{});
-  for (int it = nfull; it < ntiles; ++it) tile(it, std::true_type{});
+  for (int it = nfull; it < nit; ++it) tile(it, std::true_type{});
 
+  if constexpr (ST > 1) {   // join: sums, in stream order
+    float* const js = reinterpret_cast<float*>(dyn);
+    constexpr int PER = (D / 2 + 3) * 64;
+    float* const at = js + ((st - 1) * (4 / ST) + sub) * PER + lane;
+    __syncthreads();
+    if (st > 0) {
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) at[(dt * 16 + r) * 64] = dq[dt][r];
+      if constexpr (BIAS) {
+        at[(D / 2) * 64] = sum_pd;
+        at[(D / 2 + 1) * 64] = sum_pb;
+        at[(D / 2 + 2) * 64] = sum_pdb;
+      }
+    }
+    __syncthreads();
+    if (st > 0) return;
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) {
+      const float* const x = js + (i * (4 / ST) + sub) * PER + lane;
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[dt][r] += x[(dt * 16 + r) * 64];
+      if constexpr (BIAS) {
+        sum_pd += x[(D / 2) * 64];
+        sum_pb += x[(D / 2 + 1) * 64];
+        sum_pdb += x[(D / 2 + 2) * 64];
+      }
+    }
+  }
   if constexpr (BIAS) {
     delta = xor32_sum(sum_pd);
     sum_pb = xor32_sum(sum_pb);
@@ -624,14 +744,14 @@ NRSE_DEV void diag_add(float v, float& lo, float& hi) {
 __host__ __device__ inline long long slab_row(int bias_len) { return ((bias_len + 63) & ~63) + 192; }
 
 template <typename T, int D>
-struct KvGeo : Geo<T, D, (D * sizeof(T) > 128 ? 32 : 64)> {
+struct KvGeo : Geo<T, D, (D * (int)sizeof(T) > 128 ? 32 : 64)> {
   // bf16 at head_dim 128: the accumulators and K fill a wave's 256 registers, V's fragments stay in LDS
   static constexpr bool VLDS = sizeof(T) == 2 && D == 128;
   static constexpr int WAVES = sizeof(T) == 4 && D == 128 ? 1 : 2;   // per SIMD
 };
 
 template <typename T, int D, bool BIAS, bool CAUSAL>
-__global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const nrse_attn_packed_bwd_params p, int slices,
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>::WAVES, KvGeo<T, D>::WAVES))) void bwd_kv_kernel(const nrse_attn_packed_bwd_params p, int slices,
                                                                          float* __restrict__ sums) {
   using G = KvGeo<T, D>;
   constexpr int KT = G::KT, NT = G::NT;
@@ -646,12 +766,16 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
   const Place pl = place(nblk, p.hkv, slices);
   if (pl.block >= nblk) return;
   // a causal block's queries start at its own rows: the first block of a sequence has the most
-  Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
+  Block bl = find_block<BQ>(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
   const int tid = threadIdx.x, lane = tid & 63;
   const bool dbias = BIAS && p.dbias_vec;
-  int* const meta = dbias ? (int*)p.part + pl.block * 4 : nullptr;
+  // with a bias a slice is whole heads, or one of `parts` runs of one head's queries: each has its own row of
+  // the slab
+  const int parts = BIAS && slices > group ? slices / group : 1, piece = BIAS ? pl.g % parts : 0;
+  const bool lists = dbias && tid == 0 && pl.kvh == 0 && pl.g < parts;
+  int* const meta = dbias ? (int*)p.part + (pl.block * parts + piece) * 4 : nullptr;
   if (!bl.any) {
-    if (dbias && tid == 0 && pl.kvh == 0 && pl.g == 0) meta[1] = meta[2] = 0;
+    if (lists) meta[1] = meta[2] = 0;
     return;
   }
   const int len = bl.len;
@@ -663,11 +787,6 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
   const int kb0 = bl.row0, k0 = kb0 + w * 32, kj = k0 + m;
   const bool live = k0 < len;
   const int qt0 = CAUSAL ? kb0 / KT : 0, qtn = (len + KT - 1) / KT, nq = qtn - qt0;
-  if (dbias && tid == 0 && pl.kvh == 0 && pl.g == 0) {
-    meta[0] = kb0;
-    meta[1] = qt0 * KT;
-    meta[2] = len + 127;
-  }
   Dma<T, G> qd, od;
   qd.init((const T*)p.q + (long long)bl.seq0 * p.q_row, p.q_row, len, lane);
   od.init((const T*)p.dout + (long long)bl.seq0 * p.dout_row, p.dout_row, len, lane);
@@ -702,11 +821,18 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
       r[KT] = nrow[1];
       r[2 * KT] = nrow[2];
     }
-    if constexpr (BIAS) bv_store<G::SEG>(bv0 + buf * 4 * G::SEG, tid, nbias);
+    if constexpr (BIAS) bv_store<G::SEG>(bv0 + buf * 4 * G::SEG, tid, nbias * LOG2E);
   };
-  // this slice's share of the group's (head, query tile) pairs; of whole heads where there is a bias
+  // this slice's share of the group's (head, query tile) pairs
   const int total = group * nq;
-  const int it0 = (int)((long long)total * pl.g / slices), it1 = (int)((long long)total * (pl.g + 1) / slices);
+  int it0 = (int)((long long)total * pl.g / slices), it1 = (int)((long long)total * (pl.g + 1) / slices);
+  int qlo = qt0, qhi = qtn;
+  if (BIAS && parts > 1) {
+    qlo = qt0 + (int)((long long)nq * piece / parts);
+    qhi = qt0 + (int)((long long)nq * (piece + 1) / parts);
+    it0 = pl.g / parts * nq + qlo - qt0;
+    it1 = it0 + qhi - qlo;
+  }
   int g = it0 / nq, qt = qt0 + it0 % nq;
   if (it0 < it1) fetch(h0 + g, qt, it0 & 1);
   Dma<T, G> vd;
@@ -743,6 +869,11 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
 #pragma unroll
   for (int j = 0; j <= 2 * NT; ++j) dacc[j] = 0.f;
   constexpr int NDIAG = 132 + 16 * (2 * NT - 1);   // diagonals of a tile: 127 down to -4 - 16 (2 NT - 1)
+  if (lists) {   // the slab row's entries: diagonal kb0 + 127 - x, x from the first query on
+    meta[0] = kb0;
+    meta[1] = qlo * KT;
+    meta[2] = qlo < qhi ? min(len + 127, qhi * KT + NDIAG) : 0;
+  }
   float* const mine =
       strip0 + ((w * 2 + ((lane >> 4) & 1)) * 2 + half) * (32 * NT) + (lane & 15) + 16 * (2 * NT - 1);
   if (dbias && tid < RING) ring[tid] = 0.f;
@@ -772,7 +903,7 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
       const int x = qb + 127 - R;
       const long long ld = slab_row(p.bias_len);
       if (done && x < min((int)ld, len + 127))
-        p.part[4LL * nblk + ((long long)h * nblk + pl.block) * ld + x] = s;
+        p.part[4LL * nblk * parts + (((long long)h * nblk + pl.block) * parts + piece) * ld + x] = s;
     }
   };
   auto shed = [&](int buf) {   // what is done with this tile, to the strips
@@ -797,7 +928,7 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
       const bool next_head = qt + 1 == qtn;
       fetch(h0 + g + next_head, next_head ? qt0 : qt + 1, buf ^ 1);
     }
-    if (dbias && qt > qt0) fold(buf ^ 1, qb - KT, h0 + g, false);
+    if (dbias && qt > qt0 && it > it0) fold(buf ^ 1, qb - KT, h0 + g, false);
     if (live && (!CAUSAL || qb + KT - 1 >= k0)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -829,10 +960,10 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
           if constexpr (BIAS) {
             const float4 g4 = *reinterpret_cast<const float4*>(rb + 2 * KT + 32 * t + 8 * a);
             const float4 b4 = *reinterpret_cast<const float4*>(bcopy + buf * 4 * G::SEG + bv_pos(uj + 32 * t + 8 * a, us));
-            pr[4 * a] = fmaf(s[4 * a], c1, fmaf(g4.x * LOG2E, b4.x, -l[0]));
-            pr[4 * a + 1] = fmaf(s[4 * a + 1], c1, fmaf(g4.y * LOG2E, b4.y, -l[1]));
-            pr[4 * a + 2] = fmaf(s[4 * a + 2], c1, fmaf(g4.z * LOG2E, b4.z, -l[2]));
-            pr[4 * a + 3] = fmaf(s[4 * a + 3], c1, fmaf(g4.w * LOG2E, b4.w, -l[3]));
+            pr[4 * a] = fmaf(s[4 * a], c1, fmaf(g4.x, b4.x, -l[0]));
+            pr[4 * a + 1] = fmaf(s[4 * a + 1], c1, fmaf(g4.y, b4.y, -l[1]));
+            pr[4 * a + 2] = fmaf(s[4 * a + 2], c1, fmaf(g4.z, b4.z, -l[2]));
+            pr[4 * a + 3] = fmaf(s[4 * a + 3], c1, fmaf(g4.w, b4.w, -l[3]));
           } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c) pr[4 * a + c] = fmaf(s[4 * a + c], c1, -l[c]);
@@ -880,7 +1011,7 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
     }
     if (dbias) shed(buf);
     if (it + 1 < it1) keep(buf ^ 1);
-    if (dbias && qt + 1 == qtn) {
+    if (dbias && (qt + 1 == qtn || it + 1 == it1)) {
       // the head's last tile: fold it and the accumulators' rest, and empty the ring
       __syncthreads();
       fold(buf, qb, h0 + g, false);
@@ -921,29 +1052,36 @@ __global__ __launch_bounds__(256, (KvGeo<T, D>::WAVES)) void bwd_kv_kernel(const
     }
 }
 
-// dk, dv = the slices' f32 sums, added in order: one workgroup per block of rows and key head
+// dk, dv = the slices' f32 sums, added in order: one workgroup per 32 rows and key head, loads of four
+// slices at once
 template <typename T, int D>
 __global__ __launch_bounds__(256) void dkv_kernel(const nrse_attn_packed_bwd_params p, int slices,
                                                   const float* __restrict__ sums) {
-  const int nblk = (int)(p.rows / BQ) + p.nseq;
+  constexpr int BR = 32;
+  const int nblk = (int)(p.rows / BR) + p.nseq;
   const Place pl = place(nblk, p.hkv, 1);
   if (pl.block >= nblk) return;
-  const Block bl = find_block(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
+  const Block bl = find_block<BR>(p.cu_seqlens, p.seq_lens, p.nseq, (int)p.rows, pl.block);
   if (!bl.any) return;
-  const int n4 = min(BQ, bl.len - bl.row0) * (D / 4);
+  const int n4 = min(BR, bl.len - bl.row0) * (D / 4);
   const long long n = p.rows * p.hkv * D;
-  for (int i = threadIdx.x; i < n4; i += 256) {
-    const long long row = bl.seq0 + bl.row0 + i / (D / 4);
-    const int d = i % (D / 4) * 4;
-    const float* a = sums + (row * p.hkv + pl.kvh) * D + d;
-    float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-    for (int s = 0; s < slices; ++s) {
-      const float4 x = *reinterpret_cast<const float4*>(a + s * 2 * n), y = *reinterpret_cast<const float4*>(a + s * 2 * n + n);
-      k.x += x.x; k.y += x.y; k.z += x.z; k.w += x.w;
-      v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+  for (int i = threadIdx.x; i < 2 * n4; i += 256) {
+    const bool second = i >= n4;
+    const int j = second ? i - n4 : i;
+    const long long row = bl.seq0 + bl.row0 + j / (D / 4);
+    const int d = j % (D / 4) * 4;
+    const float* a = sums + (second ? n : 0) + (row * p.hkv + pl.kvh) * D + d;
+    f32x4 x{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < slices; s += 4) {
+      f32x4 y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[k] = *reinterpret_cast<const f32x4*>(a + min(s + k, slices - 1) * 2 * n);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (s + k < slices) x += y[k];
     }
-    store4<T>((T*)p.dk + row * p.dk_row + pl.kvh * p.dk_head + d, k.x * p.scale, k.y * p.scale, k.z * p.scale, k.w * p.scale);
-    store4<T>((T*)p.dv + row * p.dv_row + pl.kvh * p.dv_head + d, v.x, v.y, v.z, v.w);
+    if (second) store4<T>((T*)p.dv + row * p.dv_row + pl.kvh * p.dv_head + d, x[0], x[1], x[2], x[3]);
+    else store4<T>((T*)p.dk + row * p.dk_row + pl.kvh * p.dk_head + d, x[0] * p.scale, x[1] * p.scale, x[2] * p.scale, x[3] * p.scale);
   }
 }
 
@@ -1024,8 +1162,19 @@ __global__ __launch_bounds__(256) void rel_collect_kernel(const float* __restric
 }
 
 // ---------------------------------------------------------------------------------- launches
-template <typename T, int D>
-size_t lds_fwd(bool bias) { return 4 * Geo<T, D>::TILE + (bias ? 8 * Geo<T, D>::SEG * sizeof(float) : 0); }
+template <typename T, int D, int ST>
+size_t lds_q(bool bias) {
+  using G = QGeo<T, D, ST>;
+  return G::KV_LDS + (bias ? ST * 8 * G::SEG * sizeof(float) : 0);
+}
+
+// Streams of the forward and dQ kernels: one where 128-row workgroups fill the chip (256 CUs take 512 at
+// once), more where they do not.
+int q_streams(long long rows, int nseq, int hq) {
+  const long long n = (rows / BQ + nseq) * hq;
+  return n >= 700 ? 1 : 2;
+}
+
 template <typename T, int D>
 size_t lds_kv(bool bias) {
   using G = KvGeo<T, D>;
@@ -1035,40 +1184,55 @@ size_t lds_kv(bool bias) {
 
 // Slices of a key block's (head, query tile) pairs: a chip of 256 CUs takes 512 of these workgroups at
 // once, and a batch with fewer blocks x key heads is split up to 8 ways, each slice writing f32 sums that
-// dkv_kernel adds. Not below 8 pairs a slice (of an average sequence); whole heads where a bias
-// gradient is summed.
+// dkv_kernel adds. Not below 8 pairs a slice (of an average sequence).
 int kv_slices(const nrse_attn_packed_bwd_params& p) {
   const long long groups = (p.rows / BQ + p.nseq) * p.hkv, G = p.hq / p.hkv;
   const long long kt = p.head_dim * (p.dtype == NRSE_BF16 ? 2 : 4) > 128 ? 32 : 64;
   long long n = (512 + groups - 1) / groups;
   n = std::min(n, std::min(8LL, std::max(1LL, G * (p.rows / p.nseq) / kt / 8)));
-  if (p.bias_vec)
+  if (p.bias_vec && n > G) n -= n % G;   // whole heads, or equal parts of each
+  if (p.bias_vec && n <= G)
     while (G % n) --n;
   return (int)n;
+}
+int kv_parts(const nrse_attn_packed_bwd_params& p) { return std::max(1, kv_slices(p) / (p.hq / p.hkv)); }
+
+template <typename F>
+void with_streams(int st, F f) {
+  if (st == 1) f(std::integral_constant<int, 1>{});
+  else f(std::integral_constant<int, 2>{});
 }
 
 template <typename T, int D, bool BIAS, bool CAUSAL>
 void launch_fwd(const nrse_attn_packed_fwd_params& p, hipStream_t st) {
-  const long long n = grid_size(p.rows / BQ + p.nseq, p.hkv, p.hq / p.hkv);
-  hipLaunchKernelGGL((fwd_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)n), dim3(256), (lds_fwd<T, D>(BIAS)), st, p);
+  with_streams(q_streams(p.rows, p.nseq, p.hq), [&](auto s) {
+    constexpr int ST = decltype(s)::value;
+    const long long n = grid_size(p.rows / (BQ / ST) + p.nseq, p.hkv, p.hq / p.hkv);
+    hipLaunchKernelGGL((fwd_kernel<T, D, BIAS, CAUSAL, ST>), dim3((unsigned)n), dim3(256), (lds_q<T, D, ST>(BIAS)), st, p);
+  });
 }
+
 // the workspace: the bias gradient's table of blocks and slab, then the slices' sums
 long long slab_floats(const nrse_attn_packed_bwd_params& p) {
-  const long long nblk = p.rows / BQ + p.nseq;
+  const long long nblk = (p.rows / BQ + p.nseq) * kv_parts(p);
   return p.bias_vec && p.dbias_vec ? nblk * 4 + p.hq * nblk * slab_row(p.bias_len) : 0;
 }
 
 template <typename T, int D, bool BIAS, bool CAUSAL>
 void launch_bwd(const nrse_attn_packed_bwd_params& p, hipStream_t st) {
   const long long nblk = p.rows / BQ + p.nseq;
-  hipLaunchKernelGGL((bwd_q_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, p.hq / p.hkv)), dim3(256),
-                     (lds_fwd<T, D>(BIAS)), st, p);
+  with_streams(q_streams(p.rows, p.nseq, p.hq), [&](auto s) {
+    constexpr int ST = decltype(s)::value;
+    const long long n = grid_size(p.rows / (BQ / ST) + p.nseq, p.hkv, p.hq / p.hkv);
+    hipLaunchKernelGGL((bwd_q_kernel<T, D, BIAS, CAUSAL, ST>), dim3((unsigned)n), dim3(256), (lds_q<T, D, ST>(BIAS)), st, p);
+  });
   const int ns = kv_slices(p);
   float* const sums = ns > 1 ? p.part + slab_floats(p) : nullptr;
   hipLaunchKernelGGL((bwd_kv_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, ns)), dim3(256),
                      (lds_kv<T, D>(BIAS)), st, p, ns, sums);
   if (ns > 1)
-    hipLaunchKernelGGL((dkv_kernel<T, D>), dim3((unsigned)grid_size(nblk, p.hkv, 1)), dim3(256), 0, st, p, ns, sums);
+    hipLaunchKernelGGL((dkv_kernel<T, D>), dim3((unsigned)grid_size(p.rows / 32 + p.nseq, p.hkv, 1)), dim3(256), 0, st, p, ns,
+                       sums);
 }
 
 template <typename P, typename F>
@@ -1110,7 +1274,7 @@ int check_common(const char* fn, const P* p) {
   NRSE_REQUIRE(p->nseq == 0 || p->cu_seqlens, "%s: cu_seqlens is null", fn);
   NRSE_REQUIRE(!p->bias_vec || (p->bias_len > 0 && p->bias_len <= (1 << 29)), "%s: bias_len %d", fn, p->bias_len);
   NRSE_REQUIRE(p->bias_vec || !p->gate, "%s: a gate needs a bias", fn);
-  NRSE_REQUIRE(grid_size(p->rows / BQ + p->nseq, p->hkv, p->hq / p->hkv) < (1LL << 31), "%s: too many workgroups", fn);
+  NRSE_REQUIRE(grid_size(p->rows / 32 + p->nseq, p->hkv, p->hq / p->hkv) < (1LL << 31), "%s: too many workgroups", fn);
   return NRSE_OK;
 }
 #define ROWS(fn, x) \
@@ -1173,7 +1337,7 @@ extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* 
   if (p->dbias_vec) {
     const int nd = 2 * p->bias_len - 1;
     hipLaunchKernelGGL(dbias_kernel, dim3((nd + 63) / 64, p->hq), dim3(256), 0, st, p->part, p->dbias_vec,
-                       (int)(p->rows / BQ) + p->nseq, p->bias_len, p->accumulate);
+                       ((int)(p->rows / BQ) + p->nseq) * kv_parts(*p), p->bias_len, p->accumulate);
   }
   return nrse_check_launch(fn);
 }
