@@ -731,7 +731,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
 // strips (4 waves x 4 lane rows) of 32 NT, to LDS, where the next iteration adds what falls on a diagonal,
 // a thread each, in one order, into a ring; what the workgroup will not meet again leaves the ring for
 // this block's row of a slab in memory. rows of the slab are added by dbias_kernel: no atomics.
-constexpr int RING = 192;   // more than the diagonals of a tile
+constexpr int RING = 256;   // more than the diagonals of an iteration
 template <int R>
 NRSE_DEV void diag_add(float v, float& lo, float& hi) {
   if constexpr (R == 0) {
@@ -748,19 +748,33 @@ struct KvGeo : Geo<T, D, (D * (int)sizeof(T) > 128 ? 32 : 64)> {
   // bf16 at head_dim 128: the accumulators and K fill a wave's 256 registers, V's fragments stay in LDS
   static constexpr bool VLDS = sizeof(T) == 2 && D == 128;
   static constexpr int WAVES = sizeof(T) == 4 && D == 128 ? 1 : 2;   // per SIMD
+  // Streams: where a workgroup's registers and LDS leave a SIMD two waves either way (256-byte rows), 8
+  // waves in two streams of query tiles share the keys instead of two workgroups, and end in half the time
+  static constexpr int ST = D * (int)sizeof(T) == 256 ? 2 : 1;
+  using B = Geo<T, D, (D * (int)sizeof(T) > 128 ? 32 : 64)>;
+  static constexpr int W = ST * B::KT;                               // queries of an iteration
+  static constexpr int BUF = 2 * B::TILE;                            // Q and dO tile
+  static constexpr int SLOTS = 16 * (2 * B::NT + 1);                 // of a diagonal strip
+  static constexpr int NDIAG = 132 + 32 * B::NT + B::KT * (ST - 1);  // diagonals of an iteration: 127 down
+  static_assert(NDIAG <= RING, "the ring holds an iteration's diagonals");
+  // LDS: tiles [ST][2 buffers], V [4], rows [ST][2][3][KT], bias [ST][2][4][SEG], strips [2][ST][16][SLOTS], ring
+  static constexpr int V_AT = ST * 2 * BUF, ROWS_AT = V_AT + (VLDS ? 4 * B::TILE : 0),
+                       BIAS_AT = ROWS_AT + ST * 6 * B::KT * 4, STRIPS_AT = BIAS_AT + ST * 8 * B::SEG * 4,
+                       RING_AT = STRIPS_AT + 2 * ST * 16 * SLOTS * 4, END = RING_AT + RING * 4;
+  static constexpr int JOIN = ST > 1 ? 2 * 4 * (D / 2) * 64 * 4 : 0;  // the streams' dK and dV, at the end
 };
 
 template <typename T, int D, bool BIAS, bool CAUSAL>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>::WAVES, KvGeo<T, D>::WAVES))) void bwd_kv_kernel(const nrse_attn_packed_bwd_params p, int slices,
+__global__ __launch_bounds__((256 * KvGeo<T, D>::ST)) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>::WAVES, KvGeo<T, D>::WAVES))) void bwd_kv_kernel(const nrse_attn_packed_bwd_params p, int slices,
                                                                          float* __restrict__ sums) {
   using G = KvGeo<T, D>;
-  constexpr int KT = G::KT, NT = G::NT;
+  constexpr int KT = G::KT, NT = G::NT, ST = G::ST, W = G::W;
   extern __shared__ __attribute__((aligned(16))) char dyn[];
-  char* const vt0 = dyn + 4 * G::TILE;                                // [4] tiles of 32 V rows
-  float* const rows0 = reinterpret_cast<float*>(vt0 + (G::VLDS ? 4 * G::TILE : 0));  // [2][lse, delta, gate][KT]
-  float* const bv0 = rows0 + 6 * KT;                                 // [2][4][SEG]
-  float* const strip0 = bv0 + 8 * G::SEG;                            // [2][16][32 NT]
-  float* const ring = strip0 + 2 * 16 * 32 * NT;                     // [RING]
+  char* const vt0 = dyn + G::V_AT;
+  float* const rows0 = reinterpret_cast<float*>(dyn + G::ROWS_AT);
+  float* const bv0 = reinterpret_cast<float*>(dyn + G::BIAS_AT);
+  float* const strip0 = reinterpret_cast<float*>(dyn + G::STRIPS_AT);
+  float* const ring = reinterpret_cast<float*>(dyn + G::RING_AT);
   const int group = p.hq / p.hkv;
   const int nblk = (int)(p.rows / BQ) + p.nseq;
   const Place pl = place(nblk, p.hkv, slices);
@@ -780,25 +794,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
   }
   const int len = bl.len;
   if (CAUSAL) bl.row0 = (len - 1) / BQ * BQ - bl.row0;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int st = __builtin_amdgcn_readfirstlane(tid >> 8), w = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
+  const int t8 = tid & 255;
   const int m = lane & 31, half = lane >> 5;
   Lds<T, G> L;
   L.init(lane);
   const int kb0 = bl.row0, k0 = kb0 + w * 32, kj = k0 + m;
   const bool live = k0 < len;
-  const int qt0 = CAUSAL ? kb0 / KT : 0, qtn = (len + KT - 1) / KT, nq = qtn - qt0;
+  const int qt0 = CAUSAL ? kb0 / W : 0, qtn = (len + W - 1) / W, nq = qtn - qt0;
   Dma<T, G> qd, od;
   qd.init((const T*)p.q + (long long)bl.seq0 * p.q_row, p.q_row, len, lane);
   od.init((const T*)p.dout + (long long)bl.seq0 * p.dout_row, p.dout_row, len, lane);
   const int h0 = pl.kvh * group;
   const int nd = 2 * p.bias_len - 1;
   float nrow[3] = {INF, 0.f, 1.f}, nbias = 0.f;
-  auto fetch = [&](int h, int qt, int buf) {   // start bringing tile (h, qt) into LDS buffer buf
-    char* const Q = dyn + buf * 2 * G::TILE;
-    qd.issue(Q, qt * KT, w, h * p.q_head * (long long)sizeof(T));
-    od.issue(Q + G::TILE, qt * KT, w, h * p.dout_head * (long long)sizeof(T));
-    if (tid < KT) {
-      const int qi = qt * KT + tid;
+  auto fetch = [&](int h, int qt, int buf) {   // start bringing this stream's tile of (h, qt) into buffer buf
+    char* const Q = dyn + (st * 2 + buf) * G::BUF;
+    const int qb = qt * W + st * KT;
+    qd.issue(Q, qb, w, h * p.q_head * (long long)sizeof(T));
+    od.issue(Q + G::TILE, qb, w, h * p.dout_head * (long long)sizeof(T));
+    if (t8 < KT) {
+      const int qi = qb + t8;
       const long long at = h * p.rows + bl.seq0 + min(qi, len - 1);
       const float l = p.lse[at], d = p.delta[at];
       float g = 1.f;
@@ -812,16 +828,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
     }
     // segment entry u of the tile: b[kb0 - qb + 127 - u], u = query - key + 127
     if constexpr (BIAS)
-      nbias = bv_load(p.bias_vec + (long long)h * nd, nd, kb0 - qt * KT + 127 - tid + p.bias_len - 1);
+      nbias = bv_load(p.bias_vec + (long long)h * nd, nd, kb0 - qb + 127 - t8 + p.bias_len - 1);
   };
   auto keep = [&](int buf) {   // what came by registers
-    if (tid < KT) {
-      float* r = rows0 + buf * 3 * KT + tid;
+    if (t8 < KT) {
+      float* r = rows0 + (st * 2 + buf) * 3 * KT + t8;
       r[0] = nrow[0];
       r[KT] = nrow[1];
       r[2 * KT] = nrow[2];
     }
-    if constexpr (BIAS) bv_store<G::SEG>(bv0 + buf * 4 * G::SEG, tid, nbias * LOG2E);
+    if constexpr (BIAS) bv_store<G::SEG>(bv0 + (st * 2 + buf) * 4 * G::SEG, t8, nbias * LOG2E);
   };
   // this slice's share of the group's (head, query tile) pairs
   const int total = group * nq;
@@ -839,7 +855,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
   if constexpr (G::VLDS) {
     vd.init((const T*)p.v + (long long)bl.seq0 * p.v_row + pl.kvh * p.v_head, p.v_row, len, lane);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vd.issue(vt0 + i * G::TILE, kb0 + 32 * i, w);
+    for (int i = 0; i < 4; ++i)
+      if (i % ST == st) vd.issue(vt0 + i * G::TILE, kb0 + 32 * i, w);
   }
   const char* const vt = vt0 + w * G::TILE;
   u32x4 kf[G::NS], vf[G::VLDS ? 1 : G::NS];
@@ -858,7 +875,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
   keep(it0 & 1);
   const float c1 = p.scale * LOG2E;
   const int u0 = 4 * half + 127 - (w * 32 + m);
-  const float* const bcopy = bv0 + (u0 & 3) * G::SEG;
+  const float* const bcopy = bv0 + st * 8 * G::SEG + (u0 & 3) * G::SEG;
   const int uj = u0 - (u0 & 3), us = u0 & 3;
   f32x16 dk[G::DT], dv[G::DT];
 #pragma unroll
@@ -868,37 +885,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
   float dacc[2 * NT + 1];
 #pragma unroll
   for (int j = 0; j <= 2 * NT; ++j) dacc[j] = 0.f;
-  constexpr int NDIAG = 132 + 16 * (2 * NT - 1);   // diagonals of a tile: 127 down to -4 - 16 (2 NT - 1)
   if (lists) {   // the slab row's entries: diagonal kb0 + 127 - x, x from the first query on
     meta[0] = kb0;
-    meta[1] = qlo * KT;
-    meta[2] = qlo < qhi ? min(len + 127, qhi * KT + NDIAG) : 0;
+    meta[1] = qlo * W;
+    meta[2] = qlo < qhi ? min(len + 127, (qhi - 1) * W + G::NDIAG) : 0;
   }
-  float* const mine =
-      strip0 + ((w * 2 + ((lane >> 4) & 1)) * 2 + half) * (32 * NT) + (lane & 15) + 16 * (2 * NT - 1);
+  constexpr int STRIP = 16 * G::SLOTS;   // floats of a stream's strips
+  float* const mine = strip0 + st * STRIP + ((w * 2 + ((lane >> 4) & 1)) * 2 + half) * G::SLOTS + (lane & 15) + 32 * NT;
   if (dbias && tid < RING) ring[tid] = 0.f;
 
-  // the strips of one tile into the ring; diagonal R is key - query relative to (kb0, qb). Strip
-  // (b = 2 w + kr, half) holds diagonals 16 b - 4 half + slot - 16 (2 NT - 1), so R meets 2 NT strips
-  // of each half
+  // the strips of one iteration into the ring; diagonal R is key - query relative to (kb0, qb). Strip
+  // (b = 2 w + kr, half) of stream i holds diagonals 16 b - 4 half + slot - 32 NT - KT i, so R meets 2 NT + 1
+  // strips of each half and stream
   auto fold = [&](int buf, int qb, int h, bool end) {
-    const int R = tid + 128 - NDIAG;
-    if (tid < NDIAG) {
+    const int R = tid + 128 - G::NDIAG;
+    if (tid < G::NDIAG) {
       float s = 0.f;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int x = R + 4 * hf + 16 * (2 * NT - 1);
+      for (int i = 0; i < ST; ++i)
 #pragma unroll
-        for (int db = 0; db < 2 * NT; ++db) {
-          const int b = (x >> 4) - db;
-          const bool in = (unsigned)b < 8u;
-          const float y = strip0[((buf * 8 + (in ? b : 0)) * 2 + hf) * (32 * NT) + (x & 15) + 16 * db];
-          s += in ? y : 0.f;
+        for (int hf = 0; hf < 2; ++hf) {
+          const int x = R + 4 * hf + 32 * NT + KT * i;
+#pragma unroll
+          for (int db = 0; db <= 2 * NT; ++db) {
+            const int b = (x >> 4) - db;
+            const bool in = (unsigned)b < 8u;
+            const float y = strip0[(buf * ST + i) * STRIP + ((in ? b : 0) * 2 + hf) * G::SLOTS + (x & 15) + 16 * db];
+            s += in ? y : 0.f;
+          }
         }
-      }
-      float* const slot = ring + (unsigned)(kb0 - qb + R + (1 << 30)) % RING;
+      float* const slot = ring + ((kb0 - qb + R) & (RING - 1));
       s += *slot;
-      const bool done = end || R > 127 - KT;
+      const bool done = end || R > 127 - W;
       *slot = done ? 0.f : s;
       const int x = qb + 127 - R;
       const long long ld = slab_row(p.bias_len);
@@ -906,30 +924,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
         p.part[4LL * nblk * parts + (((long long)h * nblk + pl.block) * parts + piece) * ld + x] = s;
     }
   };
-  auto shed = [&](int buf) {   // what is done with this tile, to the strips
+  auto shed = [&](int buf) {   // the accumulators, to the strips
 #pragma unroll
-    for (int j = 0; j < 2 * NT; ++j) mine[buf * 16 * 32 * NT - 16 * j] = dacc[j];
-    dacc[0] = dacc[2 * NT];
-#pragma unroll
-    for (int j = 1; j <= 2 * NT; ++j) dacc[j] = 0.f;
+    for (int j = 0; j <= 2 * NT; ++j) {
+      mine[buf * ST * STRIP - 16 * j] = dacc[j];
+      dacc[j] = 0.f;
+    }
   };
 
   const bool part_block = kb0 + BQ > len;
   for (int it = it0; it < it1; ++it) {
     // (one body and a branch around the masking alone: two bodies in the loop made the compiler copy
     // the accumulators between them)
-    const bool masked = part_block || (CAUSAL && qt * KT < kb0 + BQ - 1);
-    const int buf = it & 1, qb = qt * KT;
-    char* const Qt = dyn + buf * 2 * G::TILE;
+    const int buf = it & 1, qb = qt * W + st * KT;
+    const bool masked = part_block || (CAUSAL && qb < kb0 + BQ - 1);
+    char* const Qt = dyn + (st * 2 + buf) * G::BUF;
     char* const Ot = Qt + G::TILE;
-    const float* const rb = rows0 + buf * 3 * KT + 4 * half;
+    const float* const rb = rows0 + (st * 2 + buf) * 3 * KT + 4 * half;
     wait_all_and_meet();
     if (it + 1 < it1) {
       const bool next_head = qt + 1 == qtn;
       fetch(h0 + g + next_head, next_head ? qt0 : qt + 1, buf ^ 1);
     }
-    if (dbias && qt > qt0 && it > it0) fold(buf ^ 1, qb - KT, h0 + g, false);
-    if (live && (!CAUSAL || qb + KT - 1 >= k0)) {
+    if (dbias && qt > qt0 && it > it0) fold(buf ^ 1, (qt - 1) * W, h0 + g, false);
+    if (live && (ST == 1 || qb < len) && (!CAUSAL || qb + KT - 1 >= k0)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         f32x16 s, dp;
@@ -1012,21 +1030,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
     if (dbias) shed(buf);
     if (it + 1 < it1) keep(buf ^ 1);
     if (dbias && (qt + 1 == qtn || it + 1 == it1)) {
-      // the head's last tile: fold it and the accumulators' rest, and empty the ring
+      // the head's last tile (of this slice): fold it too, and empty the ring
       __syncthreads();
-      fold(buf, qb, h0 + g, false);
-      __syncthreads();
-      shed(buf);
-      __syncthreads();
-      fold(buf, qb + KT, h0 + g, true);
-#pragma unroll
-      for (int j = 0; j <= 2 * NT; ++j) dacc[j] = 0.f;
+      fold(buf, qt * W, h0 + g, true);
     }
     if (++qt == qtn) {
       qt = qt0;
       ++g;
     }
   }
+  if constexpr (ST > 1) {
+    // join: stream 0 leaves with dK, stream 1 with dV, each the sum in stream order
+    __syncthreads();
+    float* const put = reinterpret_cast<float*>(dyn) + ((st == 0 ? 4 : 0) + w) * (D / 2) * 64 + lane;
+    const float* const get = reinterpret_cast<const float*>(dyn) + ((st == 0 ? 0 : 4) + w) * (D / 2) * 64 + lane;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) put[(dt * 16 + r) * 64] = st == 0 ? dv[dt][r] : dk[dt][r];
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (st == 0) dk[dt][r] += get[(dt * 16 + r) * 64];
+        else dv[dt][r] = get[(dt * 16 + r) * 64] + dv[dt][r];
+      }
+  }
+  const bool out_k = ST == 1 || st == 0, out_v = ST == 1 || st == 1;
   if (kj >= len) return;
   if (sums) {   // this slice's f32 sums; dkv_kernel adds the slices in order
     const long long n = p.rows * p.hkv * D;
@@ -1035,8 +1066,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
     for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        store4<float>(a + 32 * dt + 8 * i, dk[dt][4 * i], dk[dt][4 * i + 1], dk[dt][4 * i + 2], dk[dt][4 * i + 3]);
-        store4<float>(a + n + 32 * dt + 8 * i, dv[dt][4 * i], dv[dt][4 * i + 1], dv[dt][4 * i + 2], dv[dt][4 * i + 3]);
+        if (out_k) store4<float>(a + 32 * dt + 8 * i, dk[dt][4 * i], dk[dt][4 * i + 1], dk[dt][4 * i + 2], dk[dt][4 * i + 3]);
+        if (out_v) store4<float>(a + n + 32 * dt + 8 * i, dv[dt][4 * i], dv[dt][4 * i + 1], dv[dt][4 * i + 2], dv[dt][4 * i + 3]);
       }
     return;
   }
@@ -1046,9 +1077,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KvGeo<T, D>
   for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      store4<T>(dko + 32 * dt + 8 * a, dk[dt][4 * a] * p.scale, dk[dt][4 * a + 1] * p.scale, dk[dt][4 * a + 2] * p.scale,
-                dk[dt][4 * a + 3] * p.scale);
-      store4<T>(dvo + 32 * dt + 8 * a, dv[dt][4 * a], dv[dt][4 * a + 1], dv[dt][4 * a + 2], dv[dt][4 * a + 3]);
+      if (out_k)
+        store4<T>(dko + 32 * dt + 8 * a, dk[dt][4 * a] * p.scale, dk[dt][4 * a + 1] * p.scale,
+                  dk[dt][4 * a + 2] * p.scale, dk[dt][4 * a + 3] * p.scale);
+      if (out_v) store4<T>(dvo + 32 * dt + 8 * a, dv[dt][4 * a], dv[dt][4 * a + 1], dv[dt][4 * a + 2], dv[dt][4 * a + 3]);
     }
 }
 
@@ -1178,18 +1210,21 @@ int q_streams(long long rows, int nseq, int hq) {
 template <typename T, int D>
 size_t lds_kv(bool bias) {
   using G = KvGeo<T, D>;
-  return (G::VLDS ? 8 : 4) * G::TILE + 6 * G::KT * sizeof(float) +
-         (bias ? (8 * G::SEG + 2 * 16 * 32 * G::NT + RING) * sizeof(float) : 0);
+  return std::max(bias ? G::END : G::BIAS_AT, G::JOIN);
 }
 
-// Slices of a key block's (head, query tile) pairs: a chip of 256 CUs takes 512 of these workgroups at
-// once, and a batch with fewer blocks x key heads is split up to 8 ways, each slice writing f32 sums that
-// dkv_kernel adds. Not below 8 pairs a slice (of an average sequence).
+// Slices of a key block's (head, query tile) pairs: with fewer than 512 workgroups the longest of them, a
+// causal sequence's first block, decides the time, and a batch with fewer blocks x key heads is split up
+// to 8 ways, each slice writing f32 sums that dkv_kernel adds. Not below 4 pairs a slice (of an average
+// sequence; 1 in f32, whose pairs take 8 times as long). Measured: causal f32 batch of 104 groups,
+// backward 139 us in 1 slice, 105 in 2, 89 in 4; causal bf16 of 152 groups 198 us in 2, 159 in 4, 175 in 7 (the sums'
+// traffic); 944 groups 141 us in 1, 173 in 2.
 int kv_slices(const nrse_attn_packed_bwd_params& p) {
   const long long groups = (p.rows / BQ + p.nseq) * p.hkv, G = p.hq / p.hkv;
-  const long long kt = p.head_dim * (p.dtype == NRSE_BF16 ? 2 : 4) > 128 ? 32 : 64;
+  const bool f32 = p.dtype == NRSE_F32;
+  const long long pair = f32 && p.head_dim == 128 ? 32 : 64;   // queries of an iteration
   long long n = (512 + groups - 1) / groups;
-  n = std::min(n, std::min(8LL, std::max(1LL, G * (p.rows / p.nseq) / kt / 8)));
+  n = std::min(n, std::min(8LL, std::max(1LL, G * (p.rows / p.nseq) / pair / (f32 ? 1 : 4))));
   if (p.bias_vec && n > G) n -= n % G;   // whole heads, or equal parts of each
   if (p.bias_vec && n <= G)
     while (G % n) --n;
@@ -1228,8 +1263,8 @@ void launch_bwd(const nrse_attn_packed_bwd_params& p, hipStream_t st) {
   });
   const int ns = kv_slices(p);
   float* const sums = ns > 1 ? p.part + slab_floats(p) : nullptr;
-  hipLaunchKernelGGL((bwd_kv_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, ns)), dim3(256),
-                     (lds_kv<T, D>(BIAS)), st, p, ns, sums);
+  hipLaunchKernelGGL((bwd_kv_kernel<T, D, BIAS, CAUSAL>), dim3((unsigned)grid_size(nblk, p.hkv, ns)),
+                     dim3(256 * KvGeo<T, D>::ST), (lds_kv<T, D>(BIAS)), st, p, ns, sums);
   if (ns > 1)
     hipLaunchKernelGGL((dkv_kernel<T, D>), dim3((unsigned)grid_size(p.rows / 32 + p.nseq, p.hkv, 1)), dim3(256), 0, st, p, ns,
                        sums);

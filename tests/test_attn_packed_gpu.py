@@ -78,6 +78,33 @@ def test_long_sequence(nrse_device, dtype, D, causal):
     check(got, reference(q, k, v, cu, causal=causal, gate=gate, vec=vec, dout=do))
 
 
+@pytest.mark.parametrize("heads", [(1, 1), (8, 1)], ids=str)
+@pytest.mark.parametrize("bias", [None, "gated"])
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (BF16, 128), (F32, 64), (F32, 128)])
+def test_few_blocks(nrse_device, dtype, D, causal, bias, heads):
+    """One or two long sequences of few key heads: key blocks in slices and parts, streams over the keys."""
+    from nrse_amd import kernels as K
+    lens = [1400, 1] if D == 64 else [900]
+    q, k, v, do, gate, vec = data(lens, *heads, D, dtype, bias, nrse_device, 8)
+    cu = cu_of(lens, nrse_device)
+    got = run(K, q, k, v, cu, do, causal=causal, gate=gate, vec=vec)
+    check(got, reference(q, k, v, cu, causal=causal, gate=gate, vec=vec, dout=do))
+
+
+@pytest.mark.parametrize("lens", [[2048] * 3 + [333], [128] * 40 + [1]], ids=["long", "many"])
+@pytest.mark.parametrize("bias", [None, "gated"])
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (BF16, 128), (F32, 64)])
+def test_many_blocks(nrse_device, dtype, D, bias, lens):
+    """Enough blocks for one stream and one slice (the other form of each kernel)."""
+    from nrse_amd import kernels as K
+    hq = 16
+    q, k, v, do, gate, vec = data(lens, hq, hq, D, dtype, bias, nrse_device, 10)
+    cu = cu_of(lens, nrse_device)
+    got = run(K, q, k, v, cu, do, causal=True, gate=gate, vec=vec)
+    check(got, reference(q, k, v, cu, causal=True, gate=gate, vec=vec, dout=do))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
 def test_scales(nrse_device, scale):
     from nrse_amd import kernels as K
