@@ -246,13 +246,15 @@ def test_cu_seqlens_are_clamped(nrse_device):
     """Bounds past the rows, falling or negative: the sequences are what is left of them inside the tensors."""
     from nrse_amd import kernels as K
     q, k, v, do, _, _ = data([100, 100], 2, 1, 64, F32, None, nrse_device, 14)
-    want = run(K, q, k, v, cu_of([100, 100], nrse_device), do)
+    # (held to the reference, not to another call's bits: the number of sequences is part of what the order
+    # of the sums goes by)
+    ref = reference(q, k, v, cu_of([100, 100], nrse_device), causal=False, dout=do)
     for cu in ([-5, 100, 10 ** 9], [0, 100, 2 ** 31 - 1, 150, 150]):
         c = torch.tensor(cu, dtype=torch.int32, device=nrse_device)
         got = run(K, q, k, v, c, do)
-        for name in want:
-            a, b = (got[name][:, :100], want[name][:, :100]) if name == "lse" else (got[name][:100], want[name][:100])
-            assert torch.equal(a, b), name
+        for name in ref:
+            part = (slice(None), slice(0, 100)) if name == "lse" else slice(0, 100)
+            assert worst(got[name][part], tuple(x[part] for x in ref[name])) <= 1.0, name
 
 
 def test_many_sequences(nrse_device):
