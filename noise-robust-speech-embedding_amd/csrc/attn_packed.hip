@@ -267,10 +267,8 @@ NRSE_DEV float bv_load(const float* __restrict__ vec, int nd, int e) {
 template <typename T>
 NRSE_DEV void store4(T* p, float a, float b, float c, float d) {
   if constexpr (std::is_same_v<T, bf16_t>) {
-    uint2 u;
-    u.x = (uint32_t)f2bf(a) | ((uint32_t)f2bf(b) << 16);
-    u.y = (uint32_t)f2bf(c) | ((uint32_t)f2bf(d) << 16);
-    *reinterpret_cast<uint2*>(p) = u;
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<bf16x4*>(p) = bf16x4{(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
   } else {
     *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
   }
@@ -897,6 +895,10 @@ __global__ __launch_bounds__((256 * KvGeo<T, D>::ST)) __attribute__((amdgpu_wave
   // the strips of one iteration into the ring; diagonal R is key - query relative to (kb0, qb). Strip
   // (b = 2 w + kr, half) of stream i holds diagonals 16 b - 4 half + slot - 32 NT - KT i, so R meets 2 NT + 1
   // strips of each half and stream
+  float* const slab =
+      dbias ? p.part + 4LL * nblk * parts + ((long long)pl.block * parts + piece) * slab_row(p.bias_len) : nullptr;
+  const long long slab_head = (long long)nblk * parts * slab_row(p.bias_len);
+  const int xend = min((int)slab_row(p.bias_len), len + 127);
   auto fold = [&](int buf, int qb, int h, bool end) {
     const int R = tid + 128 - G::NDIAG;
     if (tid < G::NDIAG) {
@@ -919,9 +921,7 @@ __global__ __launch_bounds__((256 * KvGeo<T, D>::ST)) __attribute__((amdgpu_wave
       const bool done = end || R > 127 - W;
       *slot = done ? 0.f : s;
       const int x = qb + 127 - R;
-      const long long ld = slab_row(p.bias_len);
-      if (done && x < min((int)ld, len + 127))
-        p.part[4LL * nblk * parts + (((long long)h * nblk + pl.block) * parts + piece) * ld + x] = s;
+      if (done && x < xend) slab[h * slab_head + x] = s;
     }
   };
   auto shed = [&](int buf) {   // the accumulators, to the strips
@@ -1020,6 +1020,9 @@ __global__ __launch_bounds__((256 * KvGeo<T, D>::ST)) __attribute__((amdgpu_wave
               diag_add<2>(gg.z * ds[4 * a + 2], lo, hi);
               diag_add<3>(gg.w * ds[4 * a + 3], lo, hi);
             }
+            // (here, not sunk to where they are stored: the shifted values would all live until then, and the
+            // shifts would not fold into the additions)
+            asm volatile("" : "+v"(lo), "+v"(hi));
           }
         }
         mma_col<T, G>(L, Ot, 32 * t, pr, dv, lane);
@@ -1118,22 +1121,32 @@ __global__ __launch_bounds__(256) void dkv_kernel(const nrse_attn_packed_bwd_par
 }
 
 // dbias[h, d] (+)= the slab's rows: for each diagonal, the blocks that hold it, in block order within 4
-// quarters of the blocks, then the quarters in order.
+// quarters of the blocks, then the quarters in order. A row's place is uniform, its entry a lane's: eight
+// rows' loads at once, from a clamped entry where a row does not hold the diagonal.
 __global__ __launch_bounds__(256) void dbias_kernel(const float* __restrict__ part, float* __restrict__ dvec, int nblk,
                                                     int bias_len, int accumulate) {
   __shared__ float red[4][64];
   const int nd = 2 * bias_len - 1, h = blockIdx.y;
-  const int e = blockIdx.x * 64 + (threadIdx.x & 63), wv = threadIdx.x >> 6;
+  const int e = blockIdx.x * 64 + (threadIdx.x & 63), wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int d = e - (bias_len - 1);
-  const int* meta = (const int*)part;
+  const int4* meta = (const int4*)part;
   const long long ld = slab_row(bias_len);
   const float* slab = part + 4LL * nblk + (long long)h * nblk * ld;
   const int per = (nblk + 3) / 4, b0 = wv * per, b1 = min(nblk, b0 + per);
   float s = 0.f;
-  for (int b = b0; b < b1; ++b) {
-    const int kb = meta[4 * b], x0 = meta[4 * b + 1], x1 = meta[4 * b + 2];
-    const int x = kb + 127 - d;
-    if (x >= x0 && x < x1 && x < ld) s += slab[(long long)b * ld + x];
+  for (int b = b0; b < b1; b += 8) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = min(b + k, nblk - 1);
+      const int4 m = meta[r];
+      const int x = m.x + 127 - d;
+      const bool in = b + k < b1 && x >= m.y && x < m.z && x < ld;
+      const float y = slab[(long long)r * ld + (in ? x : 0)];
+      v[k] = in ? y : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += v[k];
   }
   red[wv][threadIdx.x & 63] = s;
   __syncthreads();
@@ -1160,37 +1173,58 @@ NRSE_DEV int bucket_of(const int* edges, int n, int rel, int causal) {
   return lo + (!causal && rel > 0 ? n : 0);
 }
 
+// (edges in LDS where they fit: a binary search through memory is 8 dependent loads)
+constexpr int EDGES = 2048;
 __global__ __launch_bounds__(256) void rel_expand_kernel(const float* __restrict__ E, const int* __restrict__ edges, int n,
                                                          float* __restrict__ vec, int H, int T, int causal) {
+  __shared__ int near[EDGES];
+  const int* at = edges;
+  if (n <= EDGES) {
+    for (int i = threadIdx.x; i < n; i += 256) near[i] = edges[i];
+    __syncthreads();
+    at = near;
+  }
   const int nd = 2 * T - 1;
-  const long long total = (long long)H * nd;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const int h = (int)(i / nd), e = (int)(i - (long long)h * nd);
-    vec[i] = E[(long long)bucket_of(edges, n, e - (T - 1), causal) * H + h];
+  for (int e = blockIdx.x * 256 + threadIdx.x; e < nd; e += gridDim.x * 256) {
+    const float* row = E + (long long)bucket_of(at, n, e - (T - 1), causal) * H;
+    for (int h = blockIdx.y; h < H; h += gridDim.y) vec[(long long)h * nd + e] = row[h];
   }
 }
 
 // dE[bucket, h] (+)= the sum of dvec[h, d] over the bucket's distances: they are one run of d (two for
-// bucket 0 of a causal table: the keys ahead count as distance 0). One wave per bucket and head, lane
-// sums 64 apart, then a fixed tree.
+// bucket 0 of a causal table: the keys ahead count as distance 0). One workgroup per bucket and head: lanes'
+// sums in distance order, then a fixed tree. The widest buckets, a whole length, set the time: 4 loads at
+// once.
 __global__ __launch_bounds__(256) void rel_collect_kernel(const float* __restrict__ dvec, const int* __restrict__ edges,
                                                           int n, float* __restrict__ dE, int H, int T, int causal,
                                                           int accumulate) {
-  const int nb = causal ? n : 2 * n;
-  const int id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (id >= nb * H) return;
-  const int b = id / H, h = id % H, k = b % n;
+  __shared__ float red[4];
+  const int b = blockIdx.x / H, h = blockIdx.x % H, k = b % n;
   const bool ahead = b >= n;
   // distances [edges[k], edges[k + 1]), at most T - 1; none at distance 0 ahead of the query
   const int d0 = max(edges[k], ahead ? 1 : 0), d1 = min(k + 1 < n ? edges[k + 1] : T, T);
   const int nd = 2 * T - 1;
   const float* row = dvec + (long long)h * nd + (T - 1);  // row[j - i]
   float s = 0.f;
-  for (int d = d0 + lane; d < d1; d += 64) s += row[ahead ? d : -d];
-  if (causal && b == 0)
-    for (int d = 1 + lane; d < T; d += 64) s += row[d];
+  auto run = [&](int from, int to, int sign) {
+    for (int d = from + (int)threadIdx.x; d < to; d += 1024) {
+      float v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = row[sign * min(d + 256 * u, T - 1)];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += d + 256 * u < to ? v[u] : 0.f;
+    }
+  };
+  run(d0, d1, ahead ? 1 : -1);
+  if (causal && b == 0) run(1, T, 1);
   s = wave_sum(s);
-  if (lane == 0) dE[(long long)b * H + h] = accumulate ? dE[(long long)b * H + h] + s : s;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const float v = red[0] + red[1] + red[2] + red[3];
+    float* o = dE + (long long)b * H + h;
+    *o = accumulate ? *o + v : v;
+  }
 }
 
 // ---------------------------------------------------------------------------------- launches
@@ -1380,10 +1414,11 @@ extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* 
 extern "C" int nrse_rel_bias_expand(const float* E, const int* edges, int n, float* vec, int H, int T, int causal,
                                     void* stream) {
   NRSE_REQUIRE(E && edges && vec && n > 0 && H > 0 && T > 0 && T <= (1 << 29), "nrse_rel_bias_expand: bad args");
-  const long long total = (long long)H * (2LL * T - 1);
-  const long long blocks = (total + 255) / 256;
-  hipLaunchKernelGGL(rel_expand_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0,
-                     (hipStream_t)stream, E, edges, n, vec, H, T, causal);
+  const long long blocks = (2LL * T - 1 + 255) / 256;
+  // a head per workgroup row while that fills the chip, all of them in one loop for a long vector
+  const unsigned rows = (unsigned)(blocks >= 1024 ? 1 : std::min(H, 65535));
+  hipLaunchKernelGGL(rel_expand_kernel, dim3((unsigned)std::min(blocks, 65536LL), rows), dim3(256), 0, (hipStream_t)stream,
+                     E, edges, n, vec, H, T, causal);
   return nrse_check_launch("nrse_rel_bias_expand");
 }
 
@@ -1392,7 +1427,7 @@ extern "C" int nrse_rel_bias_collect(const float* dvec, const int* edges, int n,
   NRSE_REQUIRE(dvec && edges && dE && n > 0 && H > 0 && T > 0 && T <= (1 << 29), "nrse_rel_bias_collect: bad args");
   const long long items = (long long)(causal ? n : 2 * n) * H;
   NRSE_REQUIRE(items < (1LL << 31), "nrse_rel_bias_collect: %lld table entries", items);
-  hipLaunchKernelGGL(rel_collect_kernel, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, (hipStream_t)stream, dvec, edges,
+  hipLaunchKernelGGL(rel_collect_kernel, dim3((unsigned)items), dim3(256), 0, (hipStream_t)stream, dvec, edges,
                      n, dE, H, T, causal, accumulate);
   return nrse_check_launch("nrse_rel_bias_collect");
 }

@@ -104,10 +104,25 @@ NRSE_DEV double parts_sum(const double* __restrict__ part, int n) {
   return block_sum(s);
 }
 
-__global__ __launch_bounds__(256) void finish_kernel(const double* __restrict__ part, int n, float* __restrict__ norm,
-                                                     double* __restrict__ exact) {
-  const double s = sqrt(parts_sum(part, n));
+// (a sum of up to 30000 chunks by one workgroup: 1024 threads, four loads each in flight)
+__global__ __launch_bounds__(1024) void finish_kernel(const double* __restrict__ part, int n, float* __restrict__ norm,
+                                                      double* __restrict__ exact) {
+  __shared__ double red[16];
+  double a = 0.0;
+  for (int i = threadIdx.x; i < n; i += 4096) {
+    double v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = part[min(i + 1024 * k, n - 1)];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a += i + 1024 * k < n ? v[k] : 0.0;
+  }
+  a = wave_sum_d(a);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int k = 0; k < 16; ++k) s += red[k];
+    s = sqrt(s);
     *norm = (float)s;
     if (exact) *exact = s;
   }
@@ -224,7 +239,7 @@ extern "C" int nrse_grad_norm(const void* const* ptrs, const long long* numel, c
   NRSE_REQUIRE(norm && part, "%s: norm or part is null", fn);
   const hipStream_t st = (hipStream_t)stream;
   if (const int rc = run_norm(fn, ptrs, numel, dtypes, count, pl, part, st)) return rc;
-  hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(256), 0, st, part, (int)pl.chunks, norm, nullptr);
+  hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(1024), 0, st, part, (int)pl.chunks, norm, nullptr);
   return nrse_check_launch(fn);
 }
 
@@ -252,7 +267,7 @@ extern "C" int nrse_clip_grad_norm(const void* const* ptrs, const long long* num
   if (const int rc = run_norm(fn, ptrs, numel, dtypes, count, pl, part, st)) return rc;
   const int few = pl.chunks > 0 && pl.chunks <= FEW ? (int)pl.chunks : 0;
   double* const exact = part + pl.chunks;
-  if (!few) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(256), 0, st, part, (int)pl.chunks, norm, exact);
+  if (!few) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(1024), 0, st, part, (int)pl.chunks, norm, exact);
   bool first = true;
   launches(ptrs, numel, dtypes, count, pl, true, [&](const Table& t, int blocks) {
     hipLaunchKernelGGL(scale_kernel, dim3(blocks), dim3(256), 0, st, t, few ? part : exact, few, first ? norm : nullptr,

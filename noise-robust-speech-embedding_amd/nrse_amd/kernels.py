@@ -7,12 +7,12 @@ from __future__ import annotations
 
 import ctypes
 import os
+from array import array
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import c_ll
 from ._lib import (AdamWParams, AttnBwdParams, AttnFwdParams, AttnPackedBwdParams, AttnPackedFwdParams, Conv0Params, GemmOperand, GemmParams, LnBwdParams,
                    LnFwdParams)
 
@@ -617,69 +617,75 @@ def attn_bwd(qkv, gate, bias, ctx, dctx, lse, delta, dqkv, dgate, diag, batch, T
 
 
 # ----------------------------------------------------------------------------- packed attention
-def _rows3(name, t, rows, heads, D, dtype, dev):
+def _rows3(fn, name, t, shape, dtype, dev):
     """(pointer, row stride, head stride) of a [rows, heads, D] operand, checked."""
-    if t.dim() != 3 or tuple(t.shape) != (rows, heads, D):
-        raise _lib.NrseError(f"{name}: shape {tuple(t.shape)}, expected {(rows, heads, D)}")
-    if t.dtype != dtype or t.device != dev:
-        raise _lib.NrseError(f"{name}: {t.dtype} on {t.device}, expected {dtype} on {dev}")
-    if D > 1 and t.stride(2) != 1:
-        raise _lib.NrseError(f"{name}: the last dimension must be contiguous (stride {t.stride(2)})")
+    if t.shape != shape or t.dtype != dtype or t.device != dev:
+        raise _lib.NrseError(f"{fn}: {name}: shape {tuple(t.shape)}, {t.dtype} on {t.device}, expected {dtype} "
+                             f"{tuple(shape)} on {dev}")
+    row, head, last = t.stride()
+    rows, heads, D = shape
+    if last != 1:
+        raise _lib.NrseError(f"{fn}: {name}: the last dimension must be contiguous (stride {last})")
     # a dimension of one element may carry any stride
-    return t.data_ptr(), t.stride(0) if rows > 1 else max(D, 8), t.stride(1) if heads > 1 else 0
+    return t.data_ptr(), row if rows > 1 else D, head if heads > 1 else 0
 
 
-def _f32(name, t, shape, dev):
+def _f32(fn, name, t, shape, dev):
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
-        raise _lib.NrseError(f"{name}: expected a contiguous float32 {tuple(shape)} on {dev}, got {t.dtype} "
+    if t.shape != shape or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
+        raise _lib.NrseError(f"{fn}: {name}: expected a contiguous float32 {tuple(shape)} on {dev}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _packed_args(fn, p, q, k, v, out, cu_seqlens, seq_lens, causal, scale, gate, bias_vec, more):
-    if not q.is_cuda:
-        raise _lib.NrseError("libnrse_hip ops take device tensors")
+def _lengths(fn, name, t, dev):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.dim() != 1 or t.device != dev or not t.is_contiguous():
+        raise _lib.NrseError(f"{fn}: {name}: expected a contiguous int32 vector on {dev}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _packed_args(fn, q, k, cu_seqlens, seq_lens, scale, gate, bias_vec):
+    """What forward and backward have in common: shapes, and the fields from cu_seqlens to bias_len in their order."""
     if q.dim() != 3 or k.dim() != 3:
         raise _lib.NrseError(f"{fn}: q and k are [rows, heads, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
-    rows, hq, D = q.shape
+    rows, hq, D = qs = q.shape
     hkv, dev, dt = k.shape[1], q.device, q.dtype
-    if dt not in (torch.bfloat16, torch.float32):
+    if not q.is_cuda:
+        raise _lib.NrseError("libnrse_hip ops take device tensors")
+    if dt != torch.bfloat16 and dt != torch.float32:
         raise _lib.NrseError(f"{fn}: dtype {dt} (bfloat16 and float32 only)")
     if hkv < 1 or hq % hkv:
         raise _lib.NrseError(f"{fn}: {hq} query heads over {hkv} key heads")
-    for name, t, h in (("q", q, hq), ("k", k, hkv), ("v", v, hkv), ("out", out, hq), *more):
-        a, r, hs = _rows3(f"{fn}: {name}", t, rows, h if h is not None else hq, D, dt, dev)
-        setattr(p, name, a)
-        setattr(p, name + "_row", r)
-        setattr(p, name + "_head", hs)
-    for name, t in (("cu_seqlens", cu_seqlens), ("seq_lens", seq_lens)):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.device != dev or not t.is_contiguous()):
-            raise _lib.NrseError(f"{fn}: {name}: expected a contiguous int32 vector on {dev}, got {t.dtype} "
-                                 f"{tuple(t.shape)} on {t.device}")
-    if cu_seqlens.numel() < 1 or (seq_lens is not None and seq_lens.numel() != cu_seqlens.numel() - 1):
-        raise _lib.NrseError(f"{fn}: {cu_seqlens.numel()} cu_seqlens, "
-                             f"{None if seq_lens is None else seq_lens.numel()} seq_lens")
-    p.cu_seqlens, p.seq_lens = cu_seqlens.data_ptr(), None if seq_lens is None else seq_lens.data_ptr()
-    p.dtype, p.rows, p.hq, p.hkv, p.head_dim = dtype_code(q), rows, hq, hkv, D
-    p.nseq, p.causal = cu_seqlens.numel() - 1, 1 if causal else 0
-    p.scale = D ** -0.5 if scale is None else scale
+    nseq = cu_seqlens.numel() - 1
+    cu, used = _lengths(fn, "cu_seqlens", cu_seqlens, dev), _lengths(fn, "seq_lens", seq_lens, dev)
+    if nseq < 0 or (used is not None and seq_lens.numel() != nseq):
+        raise _lib.NrseError(f"{fn}: {nseq + 1} cu_seqlens, {None if used is None else seq_lens.numel()} seq_lens")
+    T, vec, gt = 0, None, None
     if bias_vec is not None:
         if bias_vec.dim() != 2 or bias_vec.shape[1] % 2 == 0:
             raise _lib.NrseError(f"{fn}: bias_vec is [heads, 2 T - 1], got {tuple(bias_vec.shape)}")
-        p.bias_len = (bias_vec.shape[1] + 1) // 2
-        p.bias_vec = _f32(f"{fn}: bias_vec", bias_vec, (hq, 2 * p.bias_len - 1), dev)
-        p.gate = _f32(f"{fn}: gate", gate, (hq, rows), dev)
+        T = (bias_vec.shape[1] + 1) // 2
+        vec, gt = _f32(fn, "bias_vec", bias_vec, (hq, 2 * T - 1), dev), _f32(fn, "gate", gate, (hq, rows), dev)
     elif gate is not None:
         raise _lib.NrseError(f"{fn}: a gate needs a bias_vec")
-    return rows, hq, dev
+    return qs, torch.Size((rows, hkv, D)), dt, dev, _on(dev), (cu, used, nseq), (rows, hq, hkv, D,
+                                                                     D ** -0.5 if scale is None else scale, vec, gt, T)
+
+
+# the current stream's handle without the Stream object (stream_ptr: 2.8 us a call, this: 0.1)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: stream_ptr())
 
 
 def _on(dev):
-    """The kernels run on the current device's current stream: operands of another device are refused."""
-    if dev.index != torch.cuda.current_device():
-        raise _lib.NrseError(f"operands on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    """The current stream: the kernels run there, on the current device; operands of another are refused."""
+    here = torch.cuda.current_device()
+    if dev.index != here:
+        raise _lib.NrseError(f"operands on {dev}, the current device is cuda:{here}")
+    return _raw_stream(here)
 
 
 def attn_packed_fwd(q, k, v, cu_seqlens, out, lse=None, *, causal=False, scale=None, seq_lens=None, gate=None,
@@ -690,12 +696,15 @@ def attn_packed_fwd(q, k, v, cu_seqlens, out, lse=None, *, causal=False, scale=N
     padded batch); other rows of out and lse are left as they were. scale: default D^-1/2. lse: [hq, rows] f32 or
     None. bias_vec [hq, 2 T - 1] f32 with T >= every sequence (rel_bias_expand): + gate[h, i] * bias_vec[h, j - i +
     T - 1] on the scores; gate [hq, rows] f32 or None (1)."""
-    p = AttnPackedFwdParams()
-    rows, hq, dev = _packed_args("attn_packed_fwd", p, q, k, v, out, cu_seqlens, seq_lens, causal, scale, gate,
-                                 bias_vec, ())
-    p.lse = _f32("attn_packed_fwd: lse", lse, (hq, rows), dev)
-    _on(dev)
-    _call("nrse_attn_packed_fwd", ctypes.byref(p), stream_ptr())
+    fn = "attn_packed_fwd"
+    qs, ks, dt, dev, stream, lens, rest = _packed_args(fn, q, k, cu_seqlens, seq_lens, scale, gate, bias_vec)
+    qp, qr, qh = _rows3(fn, "q", q, qs, dt, dev)
+    kp, kr, kh = _rows3(fn, "k", k, ks, dt, dev)
+    vp, vr, vh = _rows3(fn, "v", v, ks, dt, dev)
+    op, o_r, oh = _rows3(fn, "out", out, qs, dt, dev)
+    p = AttnPackedFwdParams(_DT[dt], qp, kp, vp, op, qr, qh, kr, kh, vr, vh, o_r, oh,
+                            _f32(fn, "lse", lse, (qs[1], qs[0]), dev), *lens, 1 if causal else 0, *rest)
+    _call("nrse_attn_packed_fwd", ctypes.byref(p), stream)
 
 
 def attn_packed_bwd(q, k, v, cu_seqlens, out, dout, lse, dq, dk, dv, *, causal=False, scale=None, seq_lens=None,
@@ -703,27 +712,29 @@ def attn_packed_bwd(q, k, v, cu_seqlens, out, dout, lse, dq, dk, dv, *, causal=F
     """Backward of attn_packed_fwd: dq, dk, dv (overwritten; rows of no sequence left as they were), and with a bias
     optionally dgate [hq, rows] and dbias_vec [hq, 2 T - 1] (overwritten, or added to with accumulate: one bias shared
     by several layers). Sums in one order: the same inputs give the same bits."""
-    p = AttnPackedBwdParams()
-    rows, hq, dev = _packed_args("attn_packed_bwd", p, q, k, v, out, cu_seqlens, seq_lens, causal, scale, gate,
-                                 bias_vec, (("dout", dout, None), ("dq", dq, None), ("dk", dk, k.shape[1]),
-                                            ("dv", dv, k.shape[1])))
+    fn = "attn_packed_bwd"
+    qs, ks, dt, dev, stream, lens, rest = _packed_args(fn, q, k, cu_seqlens, seq_lens, scale, gate, bias_vec)
+    ptrs, strides = [], []
+    for name, t, shape in (("q", q, qs), ("k", k, ks), ("v", v, ks), ("out", out, qs), ("dout", dout, qs),
+                           ("dq", dq, qs), ("dk", dk, ks), ("dv", dv, ks)):
+        a, row, head = _rows3(fn, name, t, shape, dt, dev)
+        ptrs.append(a)
+        strides += (row, head)
+    rows, hq, _ = qs
     if lse is None:
-        raise _lib.NrseError("attn_packed_bwd: lse is needed")
-    p.lse = _f32("attn_packed_bwd: lse", lse, (hq, rows), dev)
+        raise _lib.NrseError(f"{fn}: lse is needed")
     if (dgate is not None and gate is None) or (dbias_vec is not None and bias_vec is None):
-        raise _lib.NrseError("attn_packed_bwd: the gradient of a gate or bias that is not there")
-    p.dgate = _f32("attn_packed_bwd: dgate", dgate, (hq, rows), dev)
-    if dbias_vec is not None:
-        p.dbias_vec = _f32("attn_packed_bwd: dbias_vec", dbias_vec, bias_vec.shape, dev)
-        p.accumulate = 1 if accumulate else 0
-    _on(dev)
+        raise _lib.NrseError(f"{fn}: the gradient of a gate or bias that is not there")
     delta = torch.empty(max(hq * rows, 1), device=dev, dtype=torch.float32)
-    p.delta = delta.data_ptr()
+    p = AttnPackedBwdParams(_DT[dt], *ptrs, *strides, _f32(fn, "lse", lse, (hq, rows), dev), delta.data_ptr(), *lens,
+                            1 if causal else 0, *rest, 1 if accumulate else 0,
+                            _f32(fn, "dgate", dgate, (hq, rows), dev),
+                            None if dbias_vec is None else _f32(fn, "dbias_vec", dbias_vec, bias_vec.shape, dev))
     n = _ws_floats("nrse_attn_packed_bwd_workspace", p)
     if n:
         ws = torch.empty(n, device=dev, dtype=torch.float32)
         p.part = ws.data_ptr()
-    _call("nrse_attn_packed_bwd", ctypes.byref(p), stream_ptr())
+    _call("nrse_attn_packed_bwd", ctypes.byref(p), stream)
 
 
 def _rel_args(fn, E, edges, vec, causal):
@@ -733,25 +744,24 @@ def _rel_args(fn, E, edges, vec, causal):
         raise _lib.NrseError(f"{fn}: vec is [heads, 2 T - 1], got {tuple(vec.shape)}")
     if edges.dtype != torch.int32 or edges.dim() != 1 or n < 1 or edges.device != vec.device or not edges.is_contiguous():
         raise _lib.NrseError(f"{fn}: edges: expected a contiguous int32 vector on {vec.device}")
-    _f32(f"{fn}: vec", vec, (H, 2 * T - 1), vec.device)
-    _f32(f"{fn}: table", E, (n if causal else 2 * n, H), vec.device)
-    _on(vec.device)
-    return H, T, n
+    _f32(fn, "vec", vec, (H, 2 * T - 1), vec.device)
+    _f32(fn, "table", E, (n if causal else 2 * n, H), vec.device)
+    return H, T, n, _on(vec.device)
 
 
 def rel_bias_expand(E, edges, vec, *, causal=False):
     """vec[h, d + T - 1] = E[bucket(d), h] for |d| < T (nrse_rel_bias_expand): the Toeplitz bias of a learned table by
     buckets, for any T from the same edges (int32 on the device, hostside.bucket_edges). E [2 n, H] two-sided, [n, H]
     causal; vec [H, 2 T - 1]."""
-    H, T, n = _rel_args("rel_bias_expand", E, edges, vec, causal)
-    _call("nrse_rel_bias_expand", ptr(E), ptr(edges), n, ptr(vec), H, T, 1 if causal else 0, stream_ptr())
+    H, T, n, stream = _rel_args("rel_bias_expand", E, edges, vec, causal)
+    _call("nrse_rel_bias_expand", ptr(E), ptr(edges), n, ptr(vec), H, T, 1 if causal else 0, stream)
 
 
 def rel_bias_collect(dvec, edges, dE, *, causal=False, accumulate=False):
     """dE[b, h] = (or +=) the sum of dvec over bucket b's distances (nrse_rel_bias_collect), in one order."""
-    H, T, n = _rel_args("rel_bias_collect", dE, edges, dvec, causal)
+    H, T, n, stream = _rel_args("rel_bias_collect", dE, edges, dvec, causal)
     _call("nrse_rel_bias_collect", ptr(dvec), ptr(edges), n, ptr(dE), H, T, 1 if causal else 0,
-          1 if accumulate else 0, stream_ptr())
+          1 if accumulate else 0, stream)
 
 
 # ----------------------------------------------------------------------------- conv front end
@@ -926,37 +936,42 @@ def sumsq(x, out):
     _call("nrse_sumsq", ptr(x), x.numel(), ptr(out), ptr(ws), stream_ptr())
 
 
+_GRAD_DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
 def _tensor_list(fn, tensors, norm):
-    """The host arrays of nrse_grad_norm: addresses, sizes and type codes, checked."""
+    """The host arrays of nrse_grad_norm (addresses, sizes and type codes, read before its call returns), checked."""
     dev = norm.device
     if not norm.is_cuda or norm.dtype != torch.float32 or norm.numel() != 1:
         raise _lib.NrseError(f"{fn}: norm is one float32 on the device, got {norm.dtype} {tuple(norm.shape)} on {dev}")
-    for t in tensors:
-        if t.dtype not in (torch.float32, torch.bfloat16) or t.device != dev or not t.is_contiguous():
-            raise _lib.NrseError(f"{fn}: expected contiguous float32 or bfloat16 tensors on {dev}, got {t.dtype} "
-                                 f"{tuple(t.shape)}, strides {t.stride()}, on {t.device}")
-    _on(dev)
-    n = len(tensors)
-    a = ((ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]), (c_ll * n)(*[t.numel() for t in tensors]),
-         (ctypes.c_int * n)(*[_DT[t.dtype] for t in tensors]), n)
+    tensors, here = list(tensors), dev.index
+    codes = [_GRAD_DT.get(t.dtype) for t in tensors]
+    bad = [t for t in tensors if not t.is_contiguous() or t.get_device() != here]
+    if bad or None in codes:
+        t = bad[0] if bad else tensors[codes.index(None)]
+        raise _lib.NrseError(f"{fn}: expected contiguous float32 or bfloat16 tensors on {dev}, got {t.dtype} "
+                             f"{tuple(t.shape)}, strides {t.stride()}, on {t.device}")
+    stream = _on(dev)
+    lists = (array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]), array("i", codes))
+    a = (*[x.buffer_info()[0] for x in lists], len(codes))
     ws = int(_lib.lib().nrse_grad_norm_workspace(*a))
     if ws < 0:
         _lib.check(ws, fn)
-    return a, torch.empty(ws, device=dev, dtype=torch.float64)
+    return lists, a, torch.empty(ws, device=dev, dtype=torch.float64), stream
 
 
 def grad_norm(tensors, norm):
     """norm[0] = sqrt(sum of squares over all tensors) (nrse_grad_norm): a sequence of contiguous f32 / bf16 device
     tensors, f64 sums in a fixed order, no host sync."""
-    a, ws = _tensor_list("grad_norm", tensors, norm)
-    _call("nrse_grad_norm", *a, norm.data_ptr(), ws.data_ptr(), stream_ptr())
+    keep, a, ws, stream = _tensor_list("grad_norm", tensors, norm)
+    _call("nrse_grad_norm", *a, norm.data_ptr(), ws.data_ptr(), stream)
 
 
 def clip_grad_norm(tensors, max_norm, norm):
     """grad_norm, then every tensor scaled in place by min(1, max_norm / (norm + 1e-6)) (nrse_clip_grad_norm): the
     many-tensor form of adamw's clip, for gradients that are not one flat buffer. Tensors that overlap are refused."""
-    a, ws = _tensor_list("clip_grad_norm", tensors, norm)
-    _call("nrse_clip_grad_norm", *a, float(max_norm), norm.data_ptr(), ws.data_ptr(), stream_ptr())
+    keep, a, ws, stream = _tensor_list("clip_grad_norm", tensors, norm)
+    _call("nrse_clip_grad_norm", *a, float(max_norm), norm.data_ptr(), ws.data_ptr(), stream)
 
 
 def adamw(p, g, m, v, shadow, *, lr, beta1, beta2, eps, weight_decay, step, max_norm, sumsq_buf, grad_scale=1.0,
