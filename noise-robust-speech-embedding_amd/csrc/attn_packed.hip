@@ -66,9 +66,12 @@ struct QGeo : Geo<T, D, tile_rows(D * (int)sizeof(T), ST)> {
 };
 
 // ---------------------------------------------------------------------------------- LDS tiles
-// Row r of a panel holds its 16-byte chunk c at position c ^ sw(r): eight consecutive rows of one
-// chunk (a b128 row read) and four rows of two chunks (a transposed read) then lie on distinct banks.
-NRSE_DEV int sw(int row) { return ((row >> 1) & 3) << 1; }
+// Row r of a panel holds its 16-byte chunk c at position c ^ sw(r), sw(r) the three bits of (r / 2) % 8 in
+// reverse. A 16-lane phase of a b128 row read takes one chunk of 8 pairs of rows, r / 2 all different
+// mod 8; a transposed read takes 4 chunks of 4 rows, and the lowest bit of r / 2, moved to the top of the
+// position, puts one pair of rows on each half of the panel: both then meet every bank once.
+// (With two bits, ((r / 2) % 4) * 2, half of the LDS cycles were conflicts.)
+NRSE_DEV int sw(int row) { return ((row & 2) << 1) | ((row & 4) >> 1) | ((row & 8) >> 3); }
 template <int KT>
 NRSE_DEV int loff(int row, int chunk) {
   return (chunk >> 3) * (KT * 128) + row * 128 + (((chunk & 7) ^ sw(row)) << 4);
@@ -81,7 +84,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 template <typename T, typename G>
 struct Lds {
   int row[4];  // row m, chunk 2 c + half of a panel, c = 0 .. 3
-  int col[2];  // inner index down the rows: bf16 see rd_col; f32: column m of row 4 half (one entry)
+  int col[4];  // inner index down the rows: bf16 see rd_col; f32 see mma_col
   NRSE_DEV void init(int lane) {
     const int m = lane & 31, half = lane >> 5;
 #pragma unroll
@@ -89,10 +92,12 @@ struct Lds {
     if constexpr (std::is_same_v<T, bf16_t>) {
       const int g = lane >> 4, i = lane & 15;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        col[e] = loff<G::KT>(4 * (g >> 1) + (i >> 2), 4 * e + 2 * (g & 1) + ((i & 3) >> 1)) + (i & 1) * 8;
+      for (int e = 0; e < 4; ++e)
+        col[e] = loff<G::KT>(4 * (g >> 1) + (i >> 2) + 8 * (e >> 1), 4 * (e & 1) + 2 * (g & 1) + ((i & 3) >> 1)) + (i & 1) * 8;
     } else {
-      col[0] = col[1] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        col[e] = (4 * half) * 128 + (((m >> 2) ^ (half << 1) ^ (e & 1) ^ ((e & 2) << 1)) << 4) + (m & 3) * 4;
     }
   }
   // 16 bytes of row 32 t + m, fragment c
@@ -100,11 +105,11 @@ struct Lds {
     return *reinterpret_cast<const u32x4*>(tile + row[c & 3] + (c >> 2) * (G::KT * 128) + 32 * t * 128);
   }
   // bf16 operand with its inner index down the rows: lane (m, half) gets column 32 dt + m of rows
-  // r0 + 4 half .. + 3 and r0 + 8 + 4 half .. + 3 (r0 a multiple of 16: the swizzle repeats every 8 rows)
+  // r0 + 4 half .. + 3 and r0 + 8 + 4 half .. + 3 (r0 a multiple of 16: the swizzle repeats every 16 rows)
   NRSE_DEV bf16x8 rd_col(const char* tile, int r0, int dt) const {
-    const char* a = tile + col[dt & 1] + (dt >> 1) * (G::KT * 128) + r0 * 128;
-    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)a);
-    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(a + 8 * 128));
+    const char* a = tile + (dt >> 1) * (G::KT * 128) + r0 * 128;
+    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(a + col[dt & 1]));
+    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(a + col[2 + (dt & 1)]));
     const short8v v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(bf16x8, v);
   }
@@ -143,13 +148,14 @@ NRSE_DEV void mma_col(const Lds<T, G>& L, const char* t, int r0, const float* p,
         acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(L.rd_col(t, r0 + 16 * ks, dt), b, acc[dt], 0, 0, 0);
     }
   } else {
-    const int m = lane & 31, half = lane >> 5;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int row = r0 + 8 * (r >> 2) + 4 * half + (r & 3);
+      // row r0 + 8 (r / 4) + 4 half + r % 4, column 32 dt + m: of the row's swizzle, half's bit is in col, the
+      // lowest bits of r / 2 and r / 4 choose one of its four
+      const int at = (r0 + 8 * (r >> 2) + (r & 3)) * 128 + L.col[((r >> 2) & 1) + (r & 2)];
 #pragma unroll
       for (int dt = 0; dt < G::DT; ++dt) {
-        const float a = *reinterpret_cast<const float*>(t + loff<G::KT>(row, 8 * dt + (m >> 2)) + (m & 3) * 4);
+        const float a = *reinterpret_cast<const float*>(t + dt * (G::KT * 128) + at);
         acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc[dt], 0, 0, 0);
       }
     }
@@ -166,13 +172,14 @@ struct Dma {
   const char* base;   // row 0 of the sequence
   long long ld;       // bytes between rows
   int len;
-  unsigned voff;
+  unsigned even, odd;   // a lane's source, in 8-row groups of even and of odd number
   NRSE_DEV void init(const void* p, long long ld_elems, int len_, int lane) {
     base = (const char*)p;
     ld = ld_elems * (long long)sizeof(T);
     len = len_;
     const int row = lane >> 3;
-    voff = (unsigned)row * (unsigned)ld + (unsigned)(((lane & 7) ^ sw(row)) << 4);
+    even = (unsigned)row * (unsigned)ld + (unsigned)(((lane & 7) ^ sw(row)) << 4);
+    odd = (unsigned)row * (unsigned)ld + (unsigned)(((lane & 7) ^ sw(row + 8)) << 4);
   }
   // head: byte offset of the head
   NRSE_DEV void issue(char* tile, int row0, int wave, long long head = 0) const {
@@ -185,7 +192,7 @@ struct Dma {
       const int k = wave * G::DMA + j;
       const int panel = k % G::PANELS, rg = k / G::PANELS;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(tile + panel * (G::KT * 128) + rg * 1024), 16,
-                                               voff + (unsigned)(rg * 8) * ldu + (unsigned)(panel * 128), 0, 0, 0);
+                                               ((rg & 1) ? odd : even) + (unsigned)(rg * 8) * ldu + (unsigned)(panel * 128), 0, 0, 0);
     }
   }
 };
@@ -375,12 +382,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int t = 0; t < G::NT; ++t) {
+      for (int t = 0; t < G::NT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sv[t][r] = 0.f;
 #pragma unroll
-        for (int c = 0; c < G::NS; ++c) mma_row<T>(L.rd_row(Kt, t, c), qf[c], sv[t]);
-      }
+      for (int c = 0; c < G::NS; ++c)   // (the pieces' products in turn: none waits for the one before it)
+#pragma unroll
+        for (int t = 0; t < G::NT; ++t) mma_row<T>(L.rd_row(Kt, t, c), qf[c], sv[t]);
       if constexpr (sizeof(T) == 2) {
         __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
