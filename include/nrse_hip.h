@@ -249,6 +249,12 @@ long long nrse_layernorm_bwd_workspace(const nrse_ln_bwd_params* p);  /* floats 
 int nrse_ln_mean_fwd(const float* h, const float* gamma, const float* beta, float* emb, float* mean, float* rstd,
                      int batch, int T, int C, float eps, float* part, void* stream);
 
+/* The same of a padded batch: emb[b] = mean over t < lens[b] of LN(h[b, t]) (lens device int32, clamped to
+ * [0, T]; zeros for 0), overwritten; frames past the length are not read. C 256, 512, 768 or 1024. part:
+ * f32 workspace of batch * ceil(T / 32) * C floats. */
+int nrse_ln_mean_lens(const float* h, const float* gamma, const float* beta, const int* lens, float* emb, int batch,
+                      int T, int C, float eps, float* part, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Gated relative-position attention, WavLMAttention ([TF]modeling_wavlm.py:147-271) with
  * F.multi_head_attention_forward / SDPA ([TORCH]functional.py:6206, 6629).

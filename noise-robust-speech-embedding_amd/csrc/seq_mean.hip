@@ -1,0 +1,82 @@
+// The final LayerNorm and time mean of a padded batch: emb[b] = mean over t < lens[b] of LN(h[b, t]), zeros
+// for an utterance of no frames. Frames past the length are not read. Memory-bound: one read of the
+// frames; a wave per frame, 32 frames a workgroup, the workgroups' sums added in frame order (no atomics).
+#include "common.h"
+
+namespace {
+
+constexpr int ROWS = 32;
+
+template <int NK>   // C = 256 NK
+__global__ __launch_bounds__(256) void chunk_kernel(const float* __restrict__ h, const float* __restrict__ gamma,
+                                                    const float* __restrict__ beta, const int* __restrict__ lens,
+                                                    float* __restrict__ part, int T, float eps) {
+  constexpr int C = 256 * NK;
+  __shared__ float red[4][C];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, b = blockIdx.y;
+  const int n = min(max(lens[b], 0), T), t0 = blockIdx.x * ROWS, t1 = min(n, t0 + ROWS);
+  if (t0 >= n) return;   // sum_kernel goes by the length too
+  float acc[NK][4];
+#pragma unroll
+  for (int k = 0; k < NK; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[k][e] = 0.f;
+  for (int t = t0 + w; t < t1; t += 4) {
+    const float* row = h + ((long long)b * T + t) * C;
+    f32x4 v[NK];
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      v[k] = *reinterpret_cast<const f32x4*>(row + (k * 64 + lane) * 4);
+      s += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
+    }
+    const float mean = wave_sum(s) / C;
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q += (v[k][e] - mean) * (v[k][e] - mean);
+    const float rstd = rsqrtf(wave_sum(q) / C + eps);
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[k][e] += (v[k][e] - mean) * rstd;
+  }
+#pragma unroll
+  for (int k = 0; k < NK; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[w][(k * 64 + lane) * 4 + e] = acc[k][e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < C; c += 256)
+    part[((long long)b * gridDim.x + blockIdx.x) * C + c] =
+        (red[0][c] + red[1][c] + red[2][c] + red[3][c]) * gamma[c] + (t1 - t0) * beta[c];
+}
+
+__global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ part, const int* __restrict__ lens,
+                                                  float* __restrict__ emb, int T, int C, int chunks) {
+  const int b = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+  const int n = min(max(lens[b], 0), T);
+  float s = 0.f;
+  for (int i = 0; i * ROWS < n; ++i) s += part[((long long)b * chunks + i) * C + c];
+  emb[(long long)b * C + c] = n > 0 ? s / n : 0.f;
+}
+
+}  // namespace
+
+extern "C" int nrse_ln_mean_lens(const float* h, const float* gamma, const float* beta, const int* lens, float* emb,
+                                 int batch, int T, int C, float eps, float* part, void* stream) {
+  const char* fn = "nrse_ln_mean_lens";
+  NRSE_REQUIRE(h && gamma && beta && lens && emb && part && batch > 0 && batch <= 65535 && T > 0, "%s: bad args", fn);
+  NRSE_REQUIRE(((uintptr_t)h & 15) == 0, "%s: h not 16-byte aligned", fn);
+  const dim3 grid((T + ROWS - 1) / ROWS, batch);
+  const hipStream_t st = (hipStream_t)stream;
+  switch (C) {
+    case 256: hipLaunchKernelGGL(chunk_kernel<1>, grid, dim3(256), 0, st, h, gamma, beta, lens, part, T, eps); break;
+    case 512: hipLaunchKernelGGL(chunk_kernel<2>, grid, dim3(256), 0, st, h, gamma, beta, lens, part, T, eps); break;
+    case 768: hipLaunchKernelGGL(chunk_kernel<3>, grid, dim3(256), 0, st, h, gamma, beta, lens, part, T, eps); break;
+    case 1024: hipLaunchKernelGGL(chunk_kernel<4>, grid, dim3(256), 0, st, h, gamma, beta, lens, part, T, eps); break;
+    default: nrse_set_error("%s: C=%d (256, 512, 768 and 1024 only)", fn, C); return NRSE_ERR_UNSUPPORTED;
+  }
+  hipLaunchKernelGGL(sum_kernel, dim3(C / 256, batch), dim3(256), 0, st, part, lens, emb, T, C, (int)grid.x);
+  return nrse_check_launch(fn);
+}

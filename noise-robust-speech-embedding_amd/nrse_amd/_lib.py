@@ -166,6 +166,7 @@ _SIGNATURES = {
     "nrse_layernorm_bwd": ([_P(LnBwdParams), c_vp], c_int),
     "nrse_layernorm_bwd_workspace": ([_P(LnBwdParams)], c_ll),
     "nrse_ln_mean_fwd": ([c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_f, c_vp, c_vp], c_int),
+    "nrse_ln_mean_lens": ([c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_f, c_vp, c_vp], c_int),
     "nrse_bias_ld": ([c_int], c_int),
     "nrse_rel_bias_fwd": ([c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp], c_int),
     "nrse_rel_bias_vec": ([c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp], c_int),

@@ -28,7 +28,7 @@ from . import kernels as K
 from . import params as PR
 from . import rng as R
 from .arch import WavLMArch
-from .hostside import bucket_runs, bucket_vector, layerdrop_decisions
+from .hostside import bucket_edges, bucket_runs, bucket_vector, layerdrop_decisions
 
 F32 = torch.float32
 # NRSE_SERIAL_TARGET=1 runs the target view and the backward weight gradients on the main
@@ -525,11 +525,15 @@ class ByolEngine:
 
     # ------------------------------------------------------------------ encoder forward
     def encoder_forward(self, W: EncoderWeights, wav: torch.Tensor, *, train: bool, fseed: int = 0, skip=None,
-                        mask_np=None, need_grad: bool = False, hidden_dtype=None):
+                        mask_np=None, need_grad: bool = False, hidden_dtype=None, flens=None):
         """WavLMModel.forward -> time-mean embedding [B, H] (f32) and the backward tape; with
         hidden_dtype, the last_hidden_state [B, T, H] in that dtype instead of the embedding
-        (src/models/encoder.py:25-32, the emotion head's input; no tape)."""
+        (src/models/encoder.py:25-32, the emotion head's input; no tape). flens (int32 [B] on the device, embedding
+        of eval mode only): each utterance's own frames. The others are cleared before the positional conv and
+        no key, query or mean of theirs is used, so a padded batch embeds as its utterances alone."""
         a = self.arch
+        if flens is not None and (train or need_grad or hidden_dtype is not None):
+            raise _lib.NrseError("lengths: the eval-mode embedding only")
         cdt = self.cdt
         dev = self.dev
         B, L = wav.shape
@@ -626,8 +630,12 @@ class ByolEngine:
             # explicit host masks (tests, replays): pinned staging -- a copy from pageable memory
             # blocks the host until the stream reaches it
             mask = torch.from_numpy(mask_np.astype(np.uint8)).pin_memory().to(dev, non_blocking=True)
+        clear = Pm.get("masked_spec_embed")
+        if flens is not None:
+            mask = (torch.arange(T, device=dev)[None] >= flens[:, None]).to(torch.uint8)
+            clear = torch.zeros(H, device=dev, dtype=F32)
         hpad = torch.empty(B, T + pk, H, device=dev, dtype=cdt)
-        K.specaug_pad(h, mask, Pm.get("masked_spec_embed"), hpad, B, T, H, pk // 2, pk - pk // 2)
+        K.specaug_pad(h, mask, clear, hpad, B, T, H, pk // 2, pk - pk // 2)
         # -------- positional conv + residual + dropout ([TF]modeling_wavlm.py:48-90, 476-483)
         h0 = torch.empty(BT, H, device=dev, dtype=F32)
         pos_pre = torch.empty(BT, H, device=dev, dtype=cdt)
@@ -644,7 +652,14 @@ class ByolEngine:
         # bf16 (MFMA) attention reads the Toeplitz vector [nh, 2T-1] (the bias depends on j - i
         # only); the f32 parity kernels read the [nh, T, Tb] table
         E_rel = Pm["encoder.layers.0.attention.rel_attn_embed.weight"]
-        if cdt == torch.bfloat16:
+        if flens is not None:
+            bias_tab = None
+            bias_vec = torch.empty(nh, 2 * T - 1, device=dev, dtype=F32)
+            K.rel_bias_expand(E_rel, self.bucket_edges(), bias_vec)
+            starts = torch.arange(0, (B + 1) * T, T, device=dev, dtype=torch.int32)
+            # (rows of no utterance stay as they are: zeros, so that nothing unwritten meets a GEMM)
+            ctx_rows = torch.zeros(BT, H, device=dev, dtype=cdt)
+        elif cdt == torch.bfloat16:
             bias_tab = None
             bias_vec = torch.empty(nh, 2 * T - 1, device=dev, dtype=F32)
             K.rel_bias_vec(E_rel, self.buckets(T), bias_vec, nh, T)
@@ -710,18 +725,29 @@ class ByolEngine:
             K.linear_fwd(x1, self.fused(W.s_flat, li, "qkv_w"), qkv, bias=self.fused(W.m_flat, li, "qkv_b"),
                          **corr(x1_8, self.fused(W.s8_flat, li, "qkv_w") if lo8 else None))
             del x1_8
-            gate = torch.empty(B, nh, T, device=dev, dtype=F32)
             at = p + "attention."
-            K.gate_fwd(x1, Pm[at + "gru_rel_pos_linear.weight"], Pm[at + "gru_rel_pos_linear.bias"],
-                       Pm[at + "gru_rel_pos_const"], gate, B, T, nh)
-            ctx = torch.empty(BT, H, device=dev, dtype=cdt)
             ctx8 = torch.empty(BT, H, device=dev, dtype=self.corr_dt) if lo8 else None
-            lse = torch.empty(B, nh, T, device=dev, dtype=F32)
-            if mask_ev is not None:
-                torch.cuda.current_stream(dev).wait_event(mask_ev)
-            # (without the mask stream the forward hashes and, for the online view, records the bits)
-            K.attn_fwd(qkv, gate, bias_tab, ctx, lse, B, T, nh, pat, R.site_seed(fseed, R.site_attn_probs(li)),
-                       bias_vec=bias_vec, drop_mask=dmask, mask_in=mask_ev is not None, ctx8=ctx8)
+            if flens is not None:
+                gate = torch.empty(nh, BT, device=dev, dtype=F32)   # one "utterance" of all rows: [heads, rows]
+                K.gate_fwd(x1, Pm[at + "gru_rel_pos_linear.weight"], Pm[at + "gru_rel_pos_linear.bias"],
+                           Pm[at + "gru_rel_pos_const"], gate, 1, BT, nh)
+                ctx, lse = ctx_rows, None
+                q, k, v = qkv.view(BT, 3, nh, a.head_dim).unbind(1)
+                K.attn_packed_fwd(q, k, v, starts, ctx.view(BT, nh, a.head_dim), seq_lens=flens, gate=gate,
+                                  bias_vec=bias_vec)
+                if ctx8 is not None:
+                    K.cast_fp8(ctx, ctx8)
+            else:
+                gate = torch.empty(B, nh, T, device=dev, dtype=F32)
+                K.gate_fwd(x1, Pm[at + "gru_rel_pos_linear.weight"], Pm[at + "gru_rel_pos_linear.bias"],
+                           Pm[at + "gru_rel_pos_const"], gate, B, T, nh)
+                ctx = torch.empty(BT, H, device=dev, dtype=cdt)
+                lse = torch.empty(B, nh, T, device=dev, dtype=F32)
+                if mask_ev is not None:
+                    torch.cuda.current_stream(dev).wait_event(mask_ev)
+                # (without the mask stream the forward hashes and, for the online view, records the bits)
+                K.attn_fwd(qkv, gate, bias_tab, ctx, lse, B, T, nh, pat, R.site_seed(fseed, R.site_attn_probs(li)),
+                           bias_vec=bias_vec, drop_mask=dmask, mask_in=mask_ev is not None, ctx8=ctx8)
             hmid = torch.empty(BT, H, device=dev, dtype=F32)
             K.linear_fwd(ctx, Ps[at + "out_proj.weight"], hmid, bias=Pm[at + "out_proj.bias"], resid=hcur, ldr=H,
                          dropout_p=php, seed=R.site_seed(fseed, R.site_attn_out(li)),
@@ -763,6 +789,10 @@ class ByolEngine:
             return y.view(B, T, H), None, executed
         # -------- final LN + time-mean shim
         emb = torch.empty(B, H, device=dev, dtype=F32)
+        if flens is not None:
+            K.ln_mean_lens(hcur.view(B, T, H), Pm["encoder.layer_norm.weight"], Pm["encoder.layer_norm.bias"], flens,
+                           emb, a.eps)
+            return emb, None, executed
         K.zero(emb)
         mf = torch.empty(BT, device=dev, dtype=F32)
         rf = torch.empty(BT, device=dev, dtype=F32)
@@ -1434,7 +1464,30 @@ class ByolEngine:
         K.byol_loss(pred, tproj, loss)
         return pred, tproj, loss
 
-    def embed(self, wav: torch.Tensor, which: str = "online") -> torch.Tensor:
+    def embed(self, wav: torch.Tensor, which: str = "online", lengths=None) -> torch.Tensor:
+        """The time-mean embedding [B, H] of wav [B, L]. lengths (samples, [B]: a sequence or an integer tensor): the
+        utterances of a padded batch, each embedded as it would be alone; what the padding holds has no
+        part in it. An utterance shorter than one frame of the conv stack gives zeros."""
         self.sync_optimizer()
-        emb, _, _ = self.encoder_forward(self.weights(which), wav, train=False)
+        flens = None if lengths is None else self.frame_lengths(lengths, wav)
+        emb, _, _ = self.encoder_forward(self.weights(which), wav, train=False, flens=flens)
         return emb
+
+    def frame_lengths(self, lengths, wav: torch.Tensor) -> torch.Tensor:
+        """int32 [B] on the device: the conv stack's frames of each utterance of `lengths` samples."""
+        n = torch.as_tensor(lengths)
+        if n.dim() != 1 or n.shape[0] != wav.shape[0] or n.dtype.is_floating_point or n.dtype == torch.bool:
+            raise _lib.NrseError(f"lengths: {wav.shape[0]} integers expected, got {n.dtype} {tuple(n.shape)}")
+        n = n.to(torch.int64)
+        if not n.is_cuda and bool(((n < 0) | (n > wav.shape[1])).any()):
+            raise _lib.NrseError(f"lengths: outside [0, {wav.shape[1]}]: {n.tolist()}")
+        n = n.clamp(0, wav.shape[1])
+        for k, s in zip(self.arch.conv_kernel, self.arch.conv_stride):
+            n = (torch.div(n - k, s, rounding_mode="floor") + 1).clamp(min=0)
+        return n.to(torch.int32).to(self.dev, non_blocking=True)
+
+    def bucket_edges(self) -> torch.Tensor:
+        """The relative-position buckets' borders, for any length (hostside.bucket_edges), on the device."""
+        if "edges" not in self._buckets:
+            self._buckets["edges"] = torch.from_numpy(bucket_edges(self.arch.num_buckets, self.arch.max_distance)).to(self.dev)
+        return self._buckets["edges"]

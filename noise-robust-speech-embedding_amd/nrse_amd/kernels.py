@@ -530,6 +530,17 @@ def ln_mean_fwd(h, gamma, beta, emb, mean, rstd, batch, T, C, eps):
           ptr(ws), stream_ptr())
 
 
+def ln_mean_lens(h, gamma, beta, lens, emb, eps):
+    """emb[b] = mean over t < lens[b] of LN(h[b, t]) (nrse_ln_mean_lens): h [B, T, C] f32, lens [B] int32 on the
+    device; frames past the length are not read, an utterance of none gives zeros."""
+    B, T, C = h.shape
+    assert h.dtype == emb.dtype == torch.float32 and h.is_contiguous() and emb.is_contiguous() and emb.shape == (B, C)
+    assert lens.dtype == torch.int32 and lens.shape == (B,) and lens.device == h.device and lens.is_contiguous()
+    assert gamma.numel() == beta.numel() == C
+    ws = workspace(B * ((T + 31) // 32) * C)
+    _call("nrse_ln_mean_lens", ptr(h), ptr(gamma), ptr(beta), ptr(lens), ptr(emb), B, T, C, eps, ptr(ws), stream_ptr())
+
+
 # ----------------------------------------------------------------------------- attention
 def bias_ld(T: int) -> int:
     """Row stride of the [H, T, Tb] relative-position bias table (nrse_bias_ld)."""

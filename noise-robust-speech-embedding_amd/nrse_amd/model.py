@@ -118,13 +118,14 @@ class WavLMEncoder(nn.Module):
         # uncached views: user code may edit these objects without touching the engine's own views
         self.model = _ParamNamespace(engine.group_views(flat, "encoder", cached=False))
 
-    def forward(self, input_values: torch.Tensor, attention_mask=None) -> torch.Tensor:
-        # [B, 1, L] -> [B, L] (encoder.py:20-21); the attention mask is ignored (encoder.py:23-25)
+    def forward(self, input_values: torch.Tensor, attention_mask=None, lengths=None) -> torch.Tensor:
+        # [B, 1, L] -> [B, L] (encoder.py:20-21); the attention mask is ignored (encoder.py:23-25);
+        # lengths (samples per utterance) embeds a padded batch as its utterances alone (engine.embed)
         if input_values.dim() == 3:
             input_values = input_values.squeeze(1)
         x = input_values.to(self.engine.dev, torch.float32).contiguous()
         with torch.no_grad():
-            return self.engine.embed(x, self.which)
+            return self.engine.embed(x, self.which, lengths=lengths)
 
 
 class BYOLSpeechModel(nn.Module):

@@ -18,7 +18,7 @@ import time
 
 import torch
 
-from . import ddp, params as PR
+from . import ddp, kernels as K, params as PR
 from .config import get_config
 from .engine import compute_mode
 from .data import create_dataloaders, seed_host_rng
@@ -48,6 +48,30 @@ class EarlyStopping:
             if self.counter >= self.patience:
                 self.early_stop = True
         return self.early_stop
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False):
+    """torch.nn.utils.clip_grad_norm_ (train_byol.py:67) over the gradients of many parameters in two passes of
+    this framework's kernels (nrse_clip_grad_norm) instead of several launches per tensor: scales them in place
+    by min(1, max_norm / (norm + 1e-6)) and returns the norm before, on the device. 2-norm, dense f32 and bf16
+    gradients on one device; error_if_nonfinite reads the norm back first."""
+    if norm_type != 2.0:
+        raise ValueError(f"norm_type {norm_type}: the 2-norm only")
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    # a dense gradient in another order of dimensions is the same values
+    grads = [g if g.is_contiguous() or not torch.ops.aten.is_non_overlapping_and_dense(g)
+             else g.as_strided((g.numel(),), (1,)) for g in grads]
+    norm = torch.empty((), device=grads[0].device, dtype=torch.float32)
+    if error_if_nonfinite:
+        K.grad_norm(grads, norm)
+        if not math.isfinite(float(norm)):
+            raise RuntimeError(f"the gradients' norm is {float(norm)}: not clipped")
+    K.clip_grad_norm(grads, max_norm, norm)
+    return norm
 
 
 class FusedAdamW(torch.optim.Optimizer):
