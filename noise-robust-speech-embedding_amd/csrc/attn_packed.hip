@@ -35,8 +35,12 @@ constexpr float RESCALE_TAU = 8.f;
 
 NRSE_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// rows of a streamed tile, for ST streams: what keeps two workgroups on a CU (one at 512-byte rows)
-constexpr int tile_rows(int row_bytes, int ST) { return ST == 1 ? (row_bytes > 256 ? 32 : 64) : ST == 2 && row_bytes == 128 ? 64 : 32; }
+// Rows of a streamed tile, for ST streams: 64 where registers and LDS leave the waves that hide its latency,
+// else 32. bf16 at head_dim 128: 32 rows let a third wave onto a SIMD (8192 causal rows, forward 280 -> 260 us;
+// 32 rows with two waves: 290). At head_dim 64, 32 rows and a fourth wave: no faster.
+constexpr int tile_rows(int row_bytes, int es, int ST) {
+  return row_bytes == 128 && ST <= 2 ? 64 : row_bytes == 256 && es == 4 && ST == 1 ? 64 : 32;
+}
 template <typename T, int D, int KT_>
 struct Geo {
   static constexpr int RB = D * (int)sizeof(T);         // bytes of a row
@@ -54,15 +58,18 @@ struct Geo {
 // and stream i takes every ST-th key tile, its running maximum, sum and output joined with the others' in
 // LDS at the end. A workgroup then has 128 / ST rows: more of them, each ST times shorter.
 template <typename T, int D, int ST>
-struct QGeo : Geo<T, D, tile_rows(D * (int)sizeof(T), ST)> {
-  using B = Geo<T, D, tile_rows(D * (int)sizeof(T), ST)>;
+struct QGeo : Geo<T, D, tile_rows(D * (int)sizeof(T), (int)sizeof(T), ST)> {
+  using B = Geo<T, D, tile_rows(D * (int)sizeof(T), (int)sizeof(T), ST)>;
   static constexpr int BR = 128 / ST;                               // rows of a workgroup
   static constexpr int SEG = ST == 1 ? 192 : ST == 2 ? 128 : 64;    // >= KT + BR - 1, in 64s
   static_assert(SEG >= B::KT + BR - 1 && SEG * ST <= 256, "a bias entry per thread");
   static constexpr int BUF = 2 * B::TILE;                           // K and V tile
   static constexpr int KV_LDS = ST * 2 * BUF;                       // [ST][2 buffers]
-  static constexpr int WAVES = ST == 1 && B::RB == 128 ? 3 : 2;     // of the forward per SIMD
-  static constexpr int Q_WAVES = B::RB > 256 ? 1 : 2;               // of dQ
+  // of the forward, per SIMD: what the registers leave (more would spill)
+  static constexpr int waves(bool bias) {
+    return ST == 1 && (B::RB == 128 || (D == 128 && sizeof(T) == 2 && !bias)) ? 3 : 2;
+  }
+  static constexpr int Q_WAVES = B::RB > 256 ? 1 : 2;               // of dQ (three at 128-byte rows: no faster)
 };
 
 // ---------------------------------------------------------------------------------- LDS tiles
@@ -289,7 +296,7 @@ NRSE_DEV void wait_all_and_meet() {
 
 // ---------------------------------------------------------------------------------- forward
 template <typename T, int D, bool BIAS, bool CAUSAL, int ST>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::WAVES, QGeo<T, D, ST>::WAVES))) void fwd_kernel(const nrse_attn_packed_fwd_params p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::waves(BIAS), QGeo<T, D, ST>::waves(BIAS)))) void fwd_kernel(const nrse_attn_packed_fwd_params p) {
   using G = QGeo<T, D, ST>;
   constexpr int KT = G::KT;
   extern __shared__ __attribute__((aligned(16))) char dyn[];
@@ -425,12 +432,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
           for (int r = 0; r < 16; ++r)
             v[t][r] = kb + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) <= last ? v[t][r] : -INF;
       }
-      float mx = v[0][0];
+      float m4[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};   // (four chains: each step waits for its last)
 #pragma unroll
       for (int t = 0; t < G::NT; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, v[t][r]);
-      mx = xor32_max(mx);
+        for (int r = 0; r < 16; r += 2) m4[(r >> 1) & 3] = fmaxf(fmaxf(m4[(r >> 1) & 3], v[t][r]), v[t][r + 1]);
+      const float mx = xor32_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
       // thr: RESCALE_TAU once the row has a reference, -inf until then (a row whose bias is -inf
       // so far has none)
       if (__builtin_amdgcn_ballot_w64(mx > thr)) {
@@ -451,13 +458,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
       }
 #pragma unroll
       for (int t = 0; t < G::NT; ++t) {
-        float part = 0.f;
+        float part[4];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           v[t][r] = exp2_(v[t][r]);
-          part += v[t][r];
+          part[r & 3] = r < 4 ? v[t][r] : part[r & 3] + v[t][r];
         }
-        lsum += part;
+        lsum += (part[0] + part[1]) + (part[2] + part[3]);
         mma_col<T, G>(L, Vt, 32 * t, v[t], o, lane);
       }
     }
