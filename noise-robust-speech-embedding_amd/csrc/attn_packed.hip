@@ -11,10 +11,11 @@
 // rows: S^T = K Q^T, so a softmax row is one lane and its neighbour 32 lanes on, and the
 // probabilities leave the accumulators as the next product's operand without a shuffle (its inner
 // index is taken in the accumulators' order: key 8 (r / 4) + 4 half + r % 4 for register r). The
-// other side streams through LDS in tiles of 64 rows (32 at 512 bytes a row) by LDS-DMA, one tile ahead.
-// A row of 32 queries per wave reads each K and V tile once for 32 columns: LDS reads
-// (2 tiles x 4 waves) and matrix cycles are then about even at head_dim 128.
+// other side streams through LDS in tiles of 64 or 32 rows by LDS-DMA, one tile ahead. Each wave reads
+// each tile once for its 32 columns: LDS reads (2 tiles x 4 waves) and matrix cycles are then about even
+// at head_dim 128.
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.h"
@@ -142,8 +143,8 @@ NRSE_DEV void mma_row(u32x4 a, u32x4 b, f32x16& acc) {
 }
 
 // acc[dt] += X^T P for a 32-row piece of the tile at `t` (rows r0 ..): X^T from the tile, P the 16
-// registers of a 32x32 accumulator (rounded to bf16 for the bf16 product: relative 2^-9 per
-// probability, as every bf16 operand)
+// registers of a 32x32 accumulator (rounded to bf16 for the bf16 product: relative 2^-8 per
+// probability at most, as every bf16 operand)
 template <typename T, typename G>
 NRSE_DEV void mma_col(const Lds<T, G>& L, const char* t, int r0, const float* p, f32x16* acc, int lane) {
   if constexpr (std::is_same_v<T, bf16_t>) {
@@ -1336,15 +1337,18 @@ void dispatch(const P& p, F f) {
   else p.head_dim == 64 ? with_bias(float{}, d64{}) : with_bias(float{}, d128{});
 }
 
-// one operand: 16-byte rows, and no row so far on that 64 of them pass 32 bits of offset
+// one operand: 16-byte rows, and no row so far on that 64 of them pass 32 bits of offset; of one that is
+// written (`rows` of them), no two elements at one address
 int check_rows(const char* fn, const char* name, const void* ptr, long long row, long long head, const int dtype, int D,
-               int heads) {
+               int heads, long long rows = 0) {
   const int es = dtype == NRSE_BF16 ? 2 : 4;
   NRSE_REQUIRE(ptr, "%s: %s is null", fn, name);
   NRSE_REQUIRE(((uintptr_t)ptr & 15) == 0 && (row * es) % 16 == 0 && (head * es) % 16 == 0,
                "%s: %s: base and strides (%lld rows, %lld heads) must be 16-byte multiples", fn, name, row, head);
   NRSE_REQUIRE(row >= D && row * es <= (1 << 24), "%s: %s: row stride %lld outside [head_dim, 2^24 bytes]", fn, name, row);
   NRSE_REQUIRE(heads == 1 || head >= D, "%s: %s: head stride %lld below head_dim", fn, name, head);
+  NRSE_REQUIRE(rows <= 1 || heads == 1 || row >= (heads - 1) * head + D || head >= (rows - 1) * row + D,
+               "%s: %s is written: its rows and heads (strides %lld, %lld) overlap", fn, name, row, head);
   return NRSE_OK;
 }
 
@@ -1358,13 +1362,27 @@ int check_common(const char* fn, const P* p) {
   NRSE_REQUIRE(p->nseq == 0 || p->cu_seqlens, "%s: cu_seqlens is null", fn);
   NRSE_REQUIRE(!p->bias_vec || (p->bias_len > 0 && p->bias_len <= (1 << 29)), "%s: bias_len %d", fn, p->bias_len);
   NRSE_REQUIRE(p->bias_vec || !p->gate, "%s: a gate needs a bias", fn);
-  NRSE_REQUIRE(grid_size(p->rows / 32 + p->nseq, p->hkv, p->hq / p->hkv) < (1LL << 31), "%s: too many workgroups", fn);
+  // a grid has fewer than 2^32 threads: 512 of dK/dV's per 128 rows, 256 of dkv_kernel's per 32
+  NRSE_REQUIRE(grid_size(p->rows / BQ + p->nseq, p->hkv, p->hq / p->hkv) < (1LL << 23) &&
+                   grid_size(p->rows / 32 + p->nseq, p->hkv, 1) < (1LL << 24),
+               "%s: too many workgroups", fn);
+  return NRSE_OK;
+}
+
+// what is written, and every other operand: an output's workgroups end while others still read
+int check_apart(const char* fn, std::initializer_list<const void*> outs, std::initializer_list<const void*> ins) {
+  for (auto o = outs.begin(); o != outs.end(); ++o) {
+    for (auto i = outs.begin(); i != o; ++i) NRSE_REQUIRE(*i != *o, "%s: two outputs at one address", fn);
+    for (const void* i : ins) NRSE_REQUIRE(i != *o, "%s: an output at an input's address", fn);
+  }
   return NRSE_OK;
 }
 #define ROWS(fn, x) \
   if (const int rc = check_rows(fn, #x, p->x, p->x##_row, p->x##_head, p->dtype, p->head_dim, p->hq)) return rc
 #define ROWS_KV(fn, x) \
   if (const int rc = check_rows(fn, #x, p->x, p->x##_row, p->x##_head, p->dtype, p->head_dim, p->hkv)) return rc
+#define ROWS_OUT(fn, x, heads) \
+  if (const int rc = check_rows(fn, #x, p->x, p->x##_row, p->x##_head, p->dtype, p->head_dim, heads, p->rows)) return rc
 
 }  // namespace
 
@@ -1376,7 +1394,8 @@ extern "C" int nrse_attn_packed_fwd(const nrse_attn_packed_fwd_params* p, void* 
   ROWS(fn, q);
   ROWS_KV(fn, k);
   ROWS_KV(fn, v);
-  ROWS(fn, out);
+  ROWS_OUT(fn, out, p->hq);
+  if (const int rc = check_apart(fn, {p->out}, {p->q, p->k, p->v})) return rc;
   dispatch(*p, [&](auto t, auto d, auto b, auto c) {
     launch_fwd<decltype(t), decltype(d)::value, decltype(b)::value, decltype(c)::value>(*p, (hipStream_t)stream);
   });
@@ -1410,11 +1429,12 @@ extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* 
   ROWS_KV(fn, v);
   ROWS(fn, out);
   ROWS(fn, dout);
-  ROWS(fn, dq);
-  ROWS_KV(fn, dk);
-  ROWS_KV(fn, dv);
+  ROWS_OUT(fn, dq, p->hq);
+  ROWS_OUT(fn, dk, p->hkv);
+  ROWS_OUT(fn, dv, p->hkv);
   NRSE_REQUIRE(p->lse && p->delta, "%s: lse and delta are needed", fn);
   NRSE_REQUIRE(p->part || nrse_attn_packed_bwd_workspace(p) == 0, "%s: part, the workspace, is null", fn);
+  if (const int rc = check_apart(fn, {p->dq, p->dk, p->dv}, {p->q, p->k, p->v, p->out, p->dout})) return rc;
   dispatch(*p, [&](auto t, auto d, auto b, auto c) {
     launch_bwd<decltype(t), decltype(d)::value, decltype(b)::value, decltype(c)::value>(*p, st);
   });
@@ -1441,7 +1461,7 @@ extern "C" int nrse_rel_bias_collect(const float* dvec, const int* edges, int n,
                                      int accumulate, void* stream) {
   NRSE_REQUIRE(dvec && edges && dE && n > 0 && H > 0 && T > 0 && T <= (1 << 29), "nrse_rel_bias_collect: bad args");
   const long long items = (long long)(causal ? n : 2 * n) * H;
-  NRSE_REQUIRE(items < (1LL << 31), "nrse_rel_bias_collect: %lld table entries", items);
+  NRSE_REQUIRE(items < (1LL << 24), "nrse_rel_bias_collect: %lld table entries", items);   // (2^32 threads)
   hipLaunchKernelGGL(rel_collect_kernel, dim3((unsigned)items), dim3(256), 0, (hipStream_t)stream, dvec, edges,
                      n, dE, H, T, causal, accumulate);
   return nrse_check_launch("nrse_rel_bias_collect");

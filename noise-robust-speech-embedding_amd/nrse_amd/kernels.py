@@ -749,10 +749,10 @@ def attn_packed_bwd(q, k, v, cu_seqlens, out, dout, lse, dq, dk, dv, *, causal=F
 
 
 def _rel_args(fn, E, edges, vec, causal):
+    if vec.dim() != 2 or vec.shape[1] % 2 == 0:
+        raise _lib.NrseError(f"{fn}: vec is [heads, 2 T - 1], got {tuple(vec.shape)}")
     H, T = vec.shape[0], (vec.shape[1] + 1) // 2
     n = edges.numel()
-    if vec.dim() != 2 or vec.shape[1] != 2 * T - 1:
-        raise _lib.NrseError(f"{fn}: vec is [heads, 2 T - 1], got {tuple(vec.shape)}")
     if edges.dtype != torch.int32 or edges.dim() != 1 or n < 1 or edges.device != vec.device or not edges.is_contiguous():
         raise _lib.NrseError(f"{fn}: edges: expected a contiguous int32 vector on {vec.device}")
     _f32(fn, "vec", vec, (H, 2 * T - 1), vec.device)

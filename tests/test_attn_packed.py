@@ -68,6 +68,40 @@ def test_backward_refusals(kw, word):
     assert word in L.nrse_last_error().decode(), L.nrse_last_error()
 
 
+def apart(make, **kw):
+    """Every operand at an address of its own."""
+    names = [n for n, _ in make()._fields_ if f"{n}_row" in dict(make()._fields_)]
+    return make(**{**{n: A + (i << 32) for i, n in enumerate(names)}, **kw})
+
+
+@pytest.mark.parametrize("make,kw", [
+    (fwd_params, dict(out="q")), (fwd_params, dict(out="v")), (bwd_params, dict(dq="q")), (bwd_params, dict(dk="k")),
+    (bwd_params, dict(dv="dout")), (bwd_params, dict(dq="out")), (bwd_params, dict(dv="dk"))])
+def test_outputs_at_another_operands_address_are_refused(make, kw):
+    L = _lib.lib()
+    p = apart(make, rows=100000, nseq=10)
+    for name, of in kw.items():
+        setattr(p, name, getattr(p, of))
+    fn = L.nrse_attn_packed_fwd if make is fwd_params else L.nrse_attn_packed_bwd
+    assert fn(ctypes.byref(p), None) < 0 and "address" in L.nrse_last_error().decode(), L.nrse_last_error()
+
+
+@pytest.mark.parametrize("make,name", [(fwd_params, "out"), (bwd_params, "dq"), (bwd_params, "dk"), (bwd_params, "dv")])
+def test_outputs_whose_rows_and_heads_overlap_are_refused(make, name):
+    L = _lib.lib()
+    p = apart(make, rows=100000, nseq=10, **{f"{name}_row": 64, f"{name}_head": 64})
+    fn = L.nrse_attn_packed_fwd if make is fwd_params else L.nrse_attn_packed_bwd
+    assert fn(ctypes.byref(p), None) < 0 and "overlap" in L.nrse_last_error().decode(), L.nrse_last_error()
+
+
+@pytest.mark.parametrize("make", [fwd_params, bwd_params])
+def test_grids_past_the_launch_limit_are_refused(make):
+    L = _lib.lib()
+    p = apart(make, rows=1 << 28, nseq=1)   # 2^21 blocks of 8 heads
+    fn = L.nrse_attn_packed_fwd if make is fwd_params else L.nrse_attn_packed_bwd
+    assert fn(ctypes.byref(p), None) < 0 and "workgroups" in L.nrse_last_error().decode(), L.nrse_last_error()
+
+
 @pytest.mark.parametrize("make", [fwd_params, bwd_params])
 @pytest.mark.parametrize("delta", [-8, 8])
 def test_struct_size_is_checked(make, delta):
@@ -108,6 +142,9 @@ def test_wrappers_take_device_tensors_only():
     cu = torch.tensor([0, 4], dtype=torch.int32)
     with pytest.raises(_lib.NrseError, match="device tensors"):
         K.attn_packed_fwd(q, k, k, cu, torch.empty_like(q))
+    for shape in ((5,), (2, 4), (1, 2, 3)):   # (not [heads, 2 T - 1])
+        with pytest.raises(_lib.NrseError, match="heads, 2 T - 1"):
+            K.rel_bias_expand(q, cu, torch.zeros(shape))
     with pytest.raises(_lib.NrseError, match="on the device"):
         K.grad_norm([q], torch.zeros(1))
     with pytest.raises(_lib.NrseError, match="on the device"):
