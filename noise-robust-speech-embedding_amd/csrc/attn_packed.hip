@@ -170,6 +170,39 @@ NRSE_DEV void mma_col(const Lds<T, G>& L, const char* t, int r0, const float* p,
   }
 }
 
+// The same with P in two bf16 parts, its upper 16 bits and the rest, for dQ: the dS of a row sum to zero, so
+// where the keys share a direction dQ is a small difference of large terms, and one rounding of each dS to
+// bf16 was most of its error (causal bf16 batch, error over norm: dQ 2.9e-3 in one part, 2.3e-3 in two, 1.7e-3
+// of it the output's own rounding). A third more matrix work in this kernel: backward + 4 %.
+template <typename T, typename G>
+NRSE_DEV void mma_col_split(const Lds<T, G>& L, const char* t, int r0, const float* p, f32x16* acc, int lane) {
+  if constexpr (std::is_same_v<T, bf16_t>) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      u32x4 hi;
+      float lo[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned a = __float_as_uint(p[8 * ks + 2 * j]), b = __float_as_uint(p[8 * ks + 2 * j + 1]);
+        hi[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        lo[2 * j] = p[8 * ks + 2 * j] - __uint_as_float(a & 0xffff0000u);
+        lo[2 * j + 1] = p[8 * ks + 2 * j + 1] - __uint_as_float(b & 0xffff0000u);
+      }
+      const bf16x8 bh = __builtin_bit_cast(bf16x8, hi), bl = pack8(lo);
+      bf16x8 a[G::DT];
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt) {
+        a[dt] = L.rd_col(t, r0 + 16 * ks, dt);
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[dt], bh, acc[dt], 0, 0, 0);
+      }
+#pragma unroll
+      for (int dt = 0; dt < G::DT; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[dt], bl, acc[dt], 0, 0, 0);
+    }
+  } else {
+    mma_col<T, G>(L, t, r0, p, acc, lane);
+  }
+}
+
 // ---------------------------------------------------------------------------------- LDS-DMA
 // A wave instruction moves 8 rows of a panel (1 KiB): lane l brings row l / 8, position l % 8, that is
 // the logical chunk (l % 8) ^ sw(row), so the swizzle goes into the source address. The descriptor
@@ -532,14 +565,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
 }
 
 // ---------------------------------------------------------------------------------- backward: dQ, dgate
-// The forward's loop with P rebuilt from lse; also delta_i, which the dK/dV kernel reads after it.
-// Without a bias delta is rowsum(dO O), from the stored output. The gradients of bias and gate are f32
-// outputs, and the rounding of a bf16 O would be all their error: there delta is summed again as
-// sum_j P dP from the f32 accumulators, and dgate = sum P dP b - delta sum P b.
+// The forward's loop with P rebuilt from lse; also delta_i, which the dK/dV kernel reads after it. Here
+// delta is rowsum(dO O), from the stored output. The gradients of bias and gate are f32 outputs, and the
+// rounding of a bf16 O would be all their error (and a quarter of dK's): for what follows delta is summed again as
+// sum_j P dP from the f32 accumulators (EXACT), and dgate = sum P dP b - delta sum P b.
 template <typename T, int D, bool BIAS, bool CAUSAL, int ST>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::Q_WAVES, QGeo<T, D, ST>::Q_WAVES))) void bwd_q_kernel(const nrse_attn_packed_bwd_params p) {
   using G = QGeo<T, D, ST>;
   constexpr int KT = G::KT;
+  constexpr bool EXACT = BIAS || sizeof(T) == 2;
   extern __shared__ __attribute__((aligned(16))) char dyn[];
   float* const bv0 = reinterpret_cast<float*>(dyn + G::KV_LDS);
   const int group = p.hq / p.hkv;
@@ -661,15 +695,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
           float e = fmaf(s[r], c1, BIAS ? fmaf(gl, b, -lse2) : -lse2);
           if constexpr (MASKED) e = kb + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) <= last ? e : -INF;
           const float pr = exp2_(e);
-          ds[r] = pr * (dp[r] - delta);
+          const float pd = pr * dp[r];
+          ds[r] = fmaf(-delta, pr, pd);
+          if constexpr (EXACT) sum_pd += pd;
           if constexpr (BIAS) {
-            const float pd = pr * dp[r];
-            sum_pd += pd;
             sum_pb = fmaf(pr, b, sum_pb);
             sum_pdb = fmaf(pd, b, sum_pdb);
           }
         }
-        mma_col<T, G>(L, Kt, 32 * t, ds, dq, lane);
+        mma_col_split<T, G>(L, Kt, 32 * t, ds, dq, lane);
       }
     }
     if constexpr (BIAS) {
@@ -690,8 +724,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
       for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) at[(dt * 16 + r) * 64] = dq[dt][r];
+      if constexpr (EXACT) at[(D / 2) * 64] = sum_pd;
       if constexpr (BIAS) {
-        at[(D / 2) * 64] = sum_pd;
         at[(D / 2 + 1) * 64] = sum_pb;
         at[(D / 2 + 2) * 64] = sum_pdb;
       }
@@ -705,15 +739,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
       for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dq[dt][r] += x[(dt * 16 + r) * 64];
+      if constexpr (EXACT) sum_pd += x[(D / 2) * 64];
       if constexpr (BIAS) {
-        sum_pd += x[(D / 2) * 64];
         sum_pb += x[(D / 2 + 1) * 64];
         sum_pdb += x[(D / 2 + 2) * 64];
       }
     }
   }
+  if constexpr (EXACT) delta = xor32_sum(sum_pd);
   if constexpr (BIAS) {
-    delta = xor32_sum(sum_pd);
     sum_pb = xor32_sum(sum_pb);
     sum_pdb = xor32_sum(sum_pdb);
   }
