@@ -383,6 +383,46 @@ def test_capture_and_replay(nrse_device):
             assert torch.equal(o[name], w[name]) and torch.equal(w2[name], w[name]), (i, name)
 
 
+@pytest.mark.parametrize("dtype,d,hq,hkv,causal", [(BF16, 64, 4, 2, False), (BF16, 128, 8, 2, True),
+                                                   (torch.float32, 64, 4, 4, True)])
+def test_a_graph_replays_with_other_lengths(nrse_device, dtype, d, hq, hkv, causal):
+    """The lengths are read on the device: a recorded call serves every batch of as many sequences and rows."""
+    from nrse_amd import kernels as K
+    lens = [120, 61, 200, 9]
+    cu = cu_of(lens, nrse_device)
+    q, k, v, do, gate, vec = data(lens, hq, hkv, d, dtype, "gated", nrse_device, 23)
+    rows, wide = q.shape[0], torch.randn(hq, 2 * 390 - 1, device=nrse_device)
+
+    def step(o):
+        kw = dict(causal=causal, gate=gate, bias_vec=wide)
+        K.attn_packed_fwd(q, k, v, cu, o["out"], o["lse"], **kw)
+        K.attn_packed_bwd(q, k, v, cu, o["out"], do, o["lse"], o["dq"], o["dk"], o["dv"], dgate=o["dgate"],
+                          dbias_vec=o["dvec"], **kw)
+
+    def buffers():
+        return dict(out=torch.empty_like(q), lse=torch.empty(hq, rows, device=nrse_device), dq=torch.empty_like(q),
+                    dk=torch.empty_like(k), dv=torch.empty_like(v), dgate=torch.empty_like(gate),
+                    dvec=torch.empty_like(wide))
+    o = buffers()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(o)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(o)
+    for other in ([390, 0, 0, 0], [1, 129, 128, 132], [0, 0, 195, 195], lens, [97, 98, 97, 98]):
+        assert sum(other) == rows
+        cu.copy_(cu_of(other, nrse_device))
+        graph.replay()
+        w = buffers()
+        step(w)
+        torch.cuda.synchronize()
+        for name in o:
+            assert torch.equal(o[name], w[name]), (other, name)
+
+
 def test_wrapper_refusals(nrse_device):
     from nrse_amd import _lib, kernels as K
     q, k, v, do, gate, vec = data([20], 4, 2, 64, BF16, "gated", nrse_device, 20)
