@@ -239,9 +239,12 @@ struct Dma {
 };
 
 // ---------------------------------------------------------------------------------- which rows
-// The blocks of all sequences are numbered from the last sequence's last block down: under a causal
-// mask a block's work grows with its place, so the long ones of a sequence go first. The grid is
-// sized from what the host knows, rows / BR + sequences, and what is left over ends at once.
+// The blocks of all sequences are numbered from the longest sequence's last block down (the longest of
+// each 64 where there are more): a block's work grows with its sequence and, under a causal mask, with its
+// place, so the long ones start first and the short ones fill the end. The grid is sized from what the host
+// knows, rows / BR + sequences, and what is left over ends at once. A lane has a sequence; where its blocks
+// begin is the sum of the longer ones', a sequence a step. (Against the batch's own order: 16 utterances,
+// backward 134 -> 116 us; 6 causal sequences, the longest first in the batch, 163 -> 155.)
 // Bounds are taken from cu_seqlens as they stand in device memory, clamped to the tensors.
 struct Block { int seq0, len, row0; bool any; };
 
@@ -250,36 +253,35 @@ NRSE_DEV Block find_block(const int* __restrict__ cu, const int* __restrict__ us
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int base = 0; base < nseq; base += 64) {
-    const int s = nseq - 1 - (base + lane);
+    const int s = base + lane, here = min(64, nseq - base);
     int start = 0, len = 0;
-    if (s >= 0) {
+    if (s < nseq) {
       start = min(max(cu[s], 0), rows);
       len = min(max(cu[s + 1], start), rows) - start;
       if (used) len = min(len, max(used[s], 0));
     }
-    const int nb = (len + BR - 1) / BR;
-    int incl = nb;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += up;
+    int first = before, all = 0;
+    for (int j = 0; j < here; ++j) {
+      const int l = __builtin_amdgcn_readlane(len, j), n = (l + BR - 1) / BR;
+      first += (l > len || (l == len && j < lane)) ? n : 0;
+      all += n;
     }
-    const unsigned long long hit = __builtin_amdgcn_ballot_w64(before + incl > want);
+    const int nb = (len + BR - 1) / BR;
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(first <= want && want < first + nb);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      const int first = before + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(nb, l);
-      const int n = __builtin_amdgcn_readlane(nb, l);
       return Block{__builtin_amdgcn_readlane(start, l), __builtin_amdgcn_readlane(len, l),
-                   (n - 1 - (want - first)) * BR, true};
+                   (__builtin_amdgcn_readlane(first + nb, l) - 1 - want) * BR, true};
     }
-    before += __builtin_amdgcn_readlane(incl, 63);
+    before += all;
   }
   return Block{0, 0, 0, false};
 }
 
 // Workgroup i runs on XCD i % 8 (each with its own L2): the XCDs share out the key heads, and where
 // there are fewer than 8 the blocks, so that the G query heads of a block and the blocks of a sequence
-// meet the same K and V in one L2.
+// meet the same K and V in one L2. The blocks, which get shorter, are dealt out to and fro, so that no XCD
+// has the longer one every time (3 causal sequences over 2 key heads, backward 227 -> 214 us).
 struct Place { int block, kvh, g; };
 __host__ __device__ inline int gcd8(int n) { return (n & 7) == 0 ? 8 : (n & 3) == 0 ? 4 : (n & 1) == 0 ? 2 : 1; }
 NRSE_DEV Place place(int nblk, int hkv, int G) {
@@ -287,7 +289,8 @@ NRSE_DEV Place place(int nblk, int hkv, int G) {
   const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
   const int per = (nblk + nsub - 1) / nsub * G;
   const int r = local % per;
-  return Place{(r / G) * nsub + xcd / gc, (xcd % gc) * (hkv / gc) + local / per, r % G};
+  const int turn = r / G, sub = xcd / gc;
+  return Place{turn * nsub + ((turn & 1) ? nsub - 1 - sub : sub), (xcd % gc) * (hkv / gc) + local / per, r % G};
 }
 inline long long grid_size(long long nblk, int hkv, int G) {
   const int gc = gcd8(hkv), nsub = 8 / gc;
