@@ -1303,10 +1303,13 @@ size_t lds_q(bool bias) {
 }
 
 // Streams of the forward and dQ kernels: one where 128-row workgroups fill the chip (256 CUs take 512 at
-// once), more where they do not.
-int q_streams(long long rows, int nseq, int hq) {
+// once), two where they do not: under a causal mask, where half of them are short, it takes more. Measured,
+// forward / backward us in one stream and in two: full, 416 workgroups at head_dim 128 30 / 141 and 38 / 140, at 64
+// 17 / 50 and 17 / 49, 608 20 / 62 and 23 / 64, 288 13 / 44 and 13 / 43; causal, 672 at 128 77 / 262 and 68 / 257,
+// 720 at 64 43 / 181 and 44 / 178, 864 at 128 109 / 404 and 112 / 412.
+int q_streams(long long rows, int nseq, int hq, int causal) {
   const long long n = (rows / BQ + nseq) * hq;
-  return n >= 700 ? 1 : 2;
+  return n >= (causal ? 700 : 400) ? 1 : 2;
 }
 
 template <typename T, int D>
@@ -1342,7 +1345,7 @@ void with_streams(int st, F f) {
 
 template <typename T, int D, bool BIAS, bool CAUSAL>
 void launch_fwd(const nrse_attn_packed_fwd_params& p, hipStream_t st) {
-  with_streams(q_streams(p.rows, p.nseq, p.hq), [&](auto s) {
+  with_streams(q_streams(p.rows, p.nseq, p.hq, p.causal), [&](auto s) {
     constexpr int ST = decltype(s)::value;
     const long long n = grid_size(p.rows / (BQ / ST) + p.nseq, p.hkv, p.hq / p.hkv);
     hipLaunchKernelGGL((fwd_kernel<T, D, BIAS, CAUSAL, ST>), dim3((unsigned)n), dim3(256), (lds_q<T, D, ST>(BIAS)), st, p);
@@ -1358,7 +1361,7 @@ long long slab_floats(const nrse_attn_packed_bwd_params& p) {
 template <typename T, int D, bool BIAS, bool CAUSAL>
 void launch_bwd(const nrse_attn_packed_bwd_params& p, hipStream_t st) {
   const long long nblk = p.rows / BQ + p.nseq;
-  with_streams(q_streams(p.rows, p.nseq, p.hq), [&](auto s) {
+  with_streams(q_streams(p.rows, p.nseq, p.hq, p.causal), [&](auto s) {
     constexpr int ST = decltype(s)::value;
     const long long n = grid_size(p.rows / (BQ / ST) + p.nseq, p.hkv, p.hq / p.hkv);
     hipLaunchKernelGGL((bwd_q_kernel<T, D, BIAS, CAUSAL, ST>), dim3((unsigned)n), dim3(256), (lds_q<T, D, ST>(BIAS)), st, p);

@@ -105,6 +105,19 @@ def test_many_blocks(nrse_device, dtype, D, bias, lens):
     check(got, reference(q, k, v, cu, causal=True, gate=gate, vec=vec, dout=do))
 
 
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("bias", [None, "gated"])
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (BF16, 128), (F32, 64), (F32, 128)])
+def test_one_stream(nrse_device, dtype, D, bias, causal):
+    """Short sequences of many heads in no order of their lengths: one stream over the keys, for every type and mask."""
+    from nrse_amd import kernels as K
+    lens = [60, 150, 0, 129, 64] * 7 + [333, 1]
+    q, k, v, do, gate, vec = data(lens, 16, 4, D, dtype, bias, nrse_device, 24)
+    cu = cu_of(lens, nrse_device)
+    got = run(K, q, k, v, cu, do, causal=causal, gate=gate, vec=vec)
+    check(got, reference(q, k, v, cu, causal=causal, gate=gate, vec=vec, dout=do))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
 def test_scales(nrse_device, scale):
     from nrse_amd import kernels as K
