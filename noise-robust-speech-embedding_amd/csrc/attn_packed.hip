@@ -243,7 +243,7 @@ struct Dma {
 // grows with its sequence and, under a causal mask, with its place, so the long ones start first and the short
 // ones fill the end. "Longest" by classes, each three quarters of the one before, of 64 sequences at a time, a
 // lane each: a place among them is a scan or two. (Against the batch's own order: 16 utterances, backward
-// 134 -> 116 us; 6 causal sequences, the longest last in that order, 163 -> 155. An exact order by 64 steps of
+// 134 -> 113 us; 6 causal sequences, the longest last in that order, 162 -> 153. An exact order by 64 steps of
 // comparing: 64 sequences of 30 rows, forward 8 -> 20 us.) The grid is sized from what the host knows, rows / BR +
 // sequences, and what is left over ends at once.
 // Bounds are taken from cu_seqlens as they stand in device memory, clamped to the tensors.
@@ -361,8 +361,8 @@ NRSE_DEV void wait_all_and_meet() {
 // Bound by the matrix units where there are rows enough (bf16): 8192 causal rows, 16 heads of 128 over 2,
 // 258-264 us = 1040-1065 TF (the matrix units busy 66 % of the time, no LDS conflicts, the rest exp and sums beside
 // them); long full sequences 1137 TF at 128, 950 at 64. Ragged batches are bound by each workgroup's own latency and
-// by the last ones to end: 4096 causal rows in 6 sequences, 16 heads of 128 over 4, 51 us; 16 utterances of 149 to
-// 599 rows, 16 heads of 64 with a bias, 34 us (matrix units 20 % busy, waves waiting 46 %). f32 is 16 times as
+// by the last ones to end: 4096 causal rows in 6 sequences, 16 heads of 128 over 4, 50 us; 16 utterances of 149 to
+// 599 rows, 16 heads of 64 with a bias, 32 us (matrix units 20 % busy, waves waiting 46 %). f32 is 16 times as
 // much matrix time a product: 1193 rows, 8 heads of 64, 32 us. A few single-token prompts: 6 us, the launch.
 template <typename T, int D, bool BIAS, bool CAUSAL, int ST>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::waves(BIAS), QGeo<T, D, ST>::waves(BIAS)))) void fwd_kernel(const nrse_attn_packed_fwd_params p) {
@@ -604,7 +604,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
 // delta is rowsum(dO O), from the stored output. The gradients of bias and gate are f32 outputs, and the
 // rounding of a bf16 O would be all their error (and a quarter of dK's): for what follows delta is summed again as
 // sum_j P dP from the f32 accumulators (EXACT), and dgate = sum P dP b - delta sum P b.
-// The forward's batches: 75 us (4096 causal rows), 53 us (utterances), 45 us (f32). It holds Q, dO, S and dP beside dQ, so
+// The forward's batches: 70 us (4096 causal rows), 51 us (utterances), 46 us (f32). It holds Q, dO, S and dP beside dQ, so
 // two waves per SIMD; what bounds it is the latency of one tile's chain of products and exponentials.
 template <typename T, int D, bool BIAS, bool CAUSAL, int ST>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::Q_WAVES, QGeo<T, D, ST>::Q_WAVES))) void bwd_q_kernel(const nrse_attn_packed_bwd_params p) {
@@ -817,9 +817,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
 // a thread each, in one order, into a ring; what the workgroup will not meet again leaves the ring for
 // this block's row of a slab in memory. rows of the slab are added by dbias_kernel: no atomics.
 //
-// Bound by latency at two waves per SIMD, and by the causal blocks' unequal lengths: the forward's batches take 93 us
-// (4096 causal rows; matrix units 31 % busy, waves waiting 46 %) + 14 us dkv_kernel, 70 us (utterances, with both the bias
-// and its gradient), 43 + 6 us (f32); long full sequences 800 TF for the whole backward at head_dim 128, 764 at 64.
+// Bound by latency at two waves per SIMD, and by the causal blocks' unequal lengths: the forward's batches take 89 us
+// (4096 causal rows; matrix units 31 % busy, waves waiting 46 %) + 14 us dkv_kernel, 69 us (utterances, with both the bias
+// and its gradient), 45 + 6 us (f32); long full sequences 800 TF for the whole backward at head_dim 128, 764 at 64.
 constexpr int RING = 256;   // more than the diagonals of an iteration
 template <int R>
 NRSE_DEV void diag_add(float v, float& lo, float& hi) {
