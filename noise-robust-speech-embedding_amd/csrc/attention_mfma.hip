@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256) NRSE_FWD_OCC void attn_fwd_kernel(const nrse_a
                                  : nullptr;
   uint32_t mnext = DM == 2 ? (uint32_t)mrow[0] : 0u;
   // Lazy rescaling in the base-2 domain: mref is the row's reference maximum, and a tile's scores
-  // are formed relative to it in two packed fmas, v = s * c1 + (gl * bias - mref) (no separate
+  // are formed relative to it in two fmas, v = s * c1 + (gl * bias - mref) (no separate
   // subtract before the exponential). Only when some lane of the wave sees a score more than
   // RESCALE_TAU above its reference (or on the first tile, where mref is not yet set) does the
   // wave shift: mref += shift, v -= shift, o and the row sum by 2^-shift. Probabilities stay

@@ -169,11 +169,8 @@ NRSE_DEV float gelu_grad_fast(float x) {
   const float cdf = x >= 0.f ? 1.0f - h : h;
   return fmaf(x * 0.39894228040143268f, e, cdf);
 }
-// Two-lane forms of the same evaluation, op for op: packed f32 instructions in the files that the
-// Makefile lists in PACKED_F32, one instruction per lane elsewhere. Used where measured faster (conv0 forward, 5%; the
-// 256x256 GEMM's register epilogue, FFN-up +1.4 % isolated in r03 -- an r02 GEMM epilogue had
-// measured 1 % slower with it); in the LN kernels and conv0 backward the packed form was neutral
-// or slower.
+// Two-lane forms of the same evaluation, op for op, one instruction per lane (no packed f32
+// instructions: see the Makefile).
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 NRSE_DEV f32x2 pk_fma(f32x2 a, f32x2 b, f32x2 c) { return __builtin_elementwise_fma(a, b, c); }
 NRSE_DEV f32x2 splat2(float v) { return f32x2{v, v}; }
@@ -193,7 +190,7 @@ NRSE_DEV f32x2 erf_fast2(f32x2 x) {
   return x * p * f32x2{__builtin_amdgcn_rcpf(q.x), __builtin_amdgcn_rcpf(q.y)};
 }
 NRSE_DEV f32x2 gelu2(f32x2 x) { return splat2(0.5f) * x * (splat2(1.0f) + erf_fast2(x * splat2(0.70710678118654752f))); }
-// gelu_grad_fast of two lanes, op for op (same values): the polynomial and products packed, rcp /
+// gelu_grad_fast of two lanes, op for op (same values): the polynomial and products in pairs, rcp /
 // exp2 / the sign select per element
 NRSE_DEV f32x2 gelu_grad2(f32x2 x) {
   const f32x2 ax = f32x2{__builtin_fabsf(x.x), __builtin_fabsf(x.y)};

@@ -35,8 +35,7 @@ NRSE_DEV void load_wT(float* wT, const float* w, int C, int k) {
   }
 }
 
-// conv0 forward: VALU-bound (10-tap conv, LN, GELU per element), so channel pairs run as
-// packed FP32 (v_pk_fma_f32 / v_pk_mul_f32): lane owns 4*NQ channels as 2*NQ pairs.
+// conv0 forward: VALU-bound (10-tap conv, LN, GELU per element): lane owns 4*NQ channels as 2*NQ pairs.
 // K10: the model's geometry (k = KMAX = 10) as a compile-time constant -- with a runtime k every
 // tap load is conditional, a branch per tap per row
 template <int NQ, bool K10>
@@ -287,7 +286,7 @@ NRSE_DEV void ld4(const void* p, int dt, long long i, float* o) {
 //  - a row is shared by C/256 waves (lane = 4 channels, 40 dW accumulators instead of 80), the
 //    two waves of a C = 512 row exchange their LN partial sums through LDS (one barrier per row,
 //    double-buffered slots), which keeps the kernel near 128 VGPRs (4 waves per SIMD);
-//  - the conv and dW FMAs run as packed fp32 (v_pk_fma_f32: two channels per instruction);
+//  - the conv and dW FMAs are written over pairs of channels;
 //  - the next row's operands (10 samples, mean / rstd, up to two col2im taps of dy) are loaded
 //    while the current row computes, the two taps into separate registers (no load -> add chain).
 
@@ -428,7 +427,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void c
         xh[h] = (y[h] - cur.mean) * cur.rstd;
         const f32x2 z = xh[h] * ga[h] + be[h];
         const f32x2 dy = h == 0 ? f32x2{dd.x, dd.y} : f32x2{dd.z, dd.w};
-        const f32x2 gg = dy * f32x2{gelu_grad_f(z.x), gelu_grad_f(z.y)};  // (packed form measured slower here)
+        const f32x2 gg = dy * f32x2{gelu_grad_f(z.x), gelu_grad_f(z.y)};
         dga[h] += gg * xh[h];
         dbe[h] += gg;
         g[h] = gg * ga[h];
@@ -666,7 +665,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
     for (int n = 0; n < NBW; ++n)
       acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, wimg[(w * NBW + n) * 64 + lane], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-    // ---- LN + GELU backward, first half, in channel pairs (n, n + 1) as packed FP32 (the dy word
+    // ---- LN + GELU backward, first half, in channel pairs (n, n + 1) (the dy word
     // of a pair holds both): gg, dgamma, dbeta, g = gg gamma and the row sums
     constexpr int NP = NBW / 2;
     f32x2 gv[NP][4], xh2[NP][4], s1[4], s2[4];

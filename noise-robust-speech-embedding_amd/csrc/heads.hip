@@ -8,6 +8,15 @@
 
 namespace {
 
+// A product rounded by itself. In the batch sums and the running mean a product and the sum it goes into are two
+// roundings, as written, whatever the compiler would fuse: these values feed themselves back from step to step
+// (the running mean) or nearly cancel (sum of dy xhat), and the bounds of the training trajectories were taken with
+// these roundings.
+NRSE_DEV float mul_rn(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 __global__ void bn_fwd_kernel(const float* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                               float* __restrict__ y, float* __restrict__ rm, float* __restrict__ rv,
                               float* __restrict__ sm, float* __restrict__ si, int rows, int C, float momentum,
@@ -23,7 +32,7 @@ __global__ void bn_fwd_kernel(const float* __restrict__ x, const float* __restri
     for (int r = 0; r < rows; ++r) { const float d = x[(long long)r * C + c] - mean; q += d * d; }
     const float var = q / rows;
     invstd = rsqrtf(var + eps);
-    if (rm) rm[c] = (1.f - momentum) * rm[c] + momentum * mean;
+    if (rm) rm[c] = mul_rn(1.f - momentum, rm[c]) + mul_rn(momentum, mean);
     if (rv) rv[c] = (1.f - momentum) * rv[c] + momentum * (rows > 1 ? q / (rows - 1) : var);
   } else {
     mean = rm[c];
@@ -52,7 +61,7 @@ __global__ void bn_bwd_kernel(const float* __restrict__ dy, const float* __restr
     float g = dy[i];
     if (relu && !(y[i] > 0.f)) g = 0.f;
     sdy += g;
-    sdyx += g * (x[i] - mean) * invstd;
+    sdyx += mul_rn(g * (x[i] - mean), invstd);
   }
   dw[c] += sdyx;
   db[c] += sdy;
@@ -62,7 +71,7 @@ __global__ void bn_bwd_kernel(const float* __restrict__ dy, const float* __restr
     float g = dy[i];
     if (relu && !(y[i] > 0.f)) g = 0.f;
     const float xh = (x[i] - mean) * invstd;
-    dx[i] = k * (rows * g - sdy - xh * sdyx);
+    dx[i] = k * (mul_rn(rows, g) - sdy - xh * sdyx);
   }
 }
 
@@ -89,7 +98,7 @@ __global__ void bn_fwd_global_kernel(const float* __restrict__ x, const float* _
   const double m = gsums[c] / (double)N;
   const double var = fmax(gsums[C + c] / (double)N - m * m, 0.0);
   const float mean = (float)m, invstd = rsqrtf((float)var + eps);
-  if (rm) rm[c] = (1.f - momentum) * rm[c] + momentum * mean;
+  if (rm) rm[c] = mul_rn(1.f - momentum, rm[c]) + mul_rn(momentum, mean);
   if (rv) rv[c] = (1.f - momentum) * rv[c] + momentum * (float)(N > 1 ? var * N / (N - 1) : var);
   sm[c] = mean;
   si[c] = invstd;
@@ -113,7 +122,7 @@ __global__ void bn_bwd_sums_kernel(const float* __restrict__ dy, const float* __
     float g = dy[i];
     if (relu && !(y[i] > 0.f)) g = 0.f;
     sdy += g;
-    sdyx += g * (x[i] - mean) * invstd;
+    sdyx += mul_rn(g * (x[i] - mean), invstd);
   }
   sums[c] = sdy;
   sums[C + c] = sdyx;
