@@ -1295,8 +1295,10 @@ __global__ __launch_bounds__(256) void rel_collect_kernel(const float* __restric
   __shared__ float red[4];
   const int b = blockIdx.x / H, h = blockIdx.x % H, k = b % n;
   const bool ahead = b >= n;
-  // distances [edges[k], edges[k + 1]), at most T - 1; none at distance 0 ahead of the query
-  const int d0 = max(edges[k], ahead ? 1 : 0), d1 = min(k + 1 < n ? edges[k + 1] : T, T);
+  // distances [edges[k], edges[k + 1]), the first bucket's from 0 (as expand's search has it), at most T - 1; none at
+  // distance 0 ahead of the query. Both ends are clamped before anything is added to them: a border may be any
+  // int, 2^31 - 1 among them (a bucket past every length), and then the run is empty.
+  const int d0 = k == 0 ? (ahead ? 1 : 0) : min(max(edges[k], ahead ? 1 : 0), T), d1 = min(k + 1 < n ? edges[k + 1] : T, T);
   const int nd = 2 * T - 1;
   const float* row = dvec + (long long)h * nd + (T - 1);  // row[j - i]
   float s = 0.f;

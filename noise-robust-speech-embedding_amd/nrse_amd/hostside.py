@@ -45,7 +45,7 @@ def bucket_runs(bucket: np.ndarray, nb: int) -> tuple[np.ndarray, np.ndarray]:
 def bucket_edges(num_buckets: int = 320, max_distance: int = 800, causal: bool = False) -> np.ndarray:
     """int32 [n]: the smallest distance of each bucket of one side, ascending from 0 (n = num_buckets / 2 two-sided,
     num_buckets causal): bucket_vector's buckets as borders, for rel_bias_expand / rel_bias_collect. A bucket that
-    no distance falls in repeats its successor's border (or, at the top, ends past every length)."""
+    no distance falls in repeats its successor's border; the last one holds max_distance, so every border is found."""
     n = num_buckets if causal else num_buckets // 2
     if n < 2 or max_distance <= n // 2:
         raise ValueError(f"{num_buckets} buckets up to distance {max_distance}")
@@ -57,8 +57,7 @@ def bucket_edges(num_buckets: int = 320, max_distance: int = 800, causal: bool =
     lg = (lg * np.float32(n - max_exact)).astype(np.float32)
     large = np.minimum(max_exact + np.where(np.isfinite(lg), lg, 0).astype(np.int64), n - 1)
     of = np.where(rp < max_exact, rp, large)
-    edges = np.searchsorted(of, np.arange(n), side="left")
-    return np.where(edges > max_distance + 1, np.iinfo(np.int32).max, edges).astype(np.int32)
+    return np.searchsorted(of, np.arange(n), side="left").astype(np.int32)
 
 
 def compute_mask_indices(rng: np.random.Generator, batch: int, T: int, mask_prob: float, mask_length: int,
