@@ -1286,7 +1286,7 @@ __global__ __launch_bounds__(256) void rel_expand_kernel(const float* __restrict
 }
 
 // dE[bucket, h] (+)= the sum of dvec[h, d] over the bucket's distances: they are one run of d (two for
-// bucket 0 of a causal table: the keys ahead count as distance 0). One workgroup per bucket and head: lanes'
+// distance 0's bucket of a causal table: the keys ahead count as distance 0). One workgroup per bucket and head: lanes'
 // sums in distance order, then a fixed tree. The widest buckets, a whole length, set the time: 4 loads at
 // once (2500 distances, 8 heads: 13 us one at a time, 4.7 four).
 __global__ __launch_bounds__(256) void rel_collect_kernel(const float* __restrict__ dvec, const int* __restrict__ edges,
@@ -1312,7 +1312,7 @@ __global__ __launch_bounds__(256) void rel_collect_kernel(const float* __restric
     }
   };
   run(d0, d1, ahead ? 1 : -1);
-  if (causal && b == 0) run(1, T, 1);
+  if (causal && d0 == 0 && d1 > 0) run(1, T, 1);   // the bucket that holds distance 0
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();

@@ -11,7 +11,7 @@ U = 2.0 ** -24
 
 @pytest.mark.parametrize("causal", [False, True], ids=["two-sided", "causal"])
 @pytest.mark.parametrize("T", [1, 40, 700])
-@pytest.mark.parametrize("edges", [[0, 3, 9, MAX], [0, 5, MAX - 255, MAX - 254, MAX - 1, MAX, MAX], [0, MAX], [0, 1, 2, 2, 40, 700, 701],
+@pytest.mark.parametrize("edges", [[0, 3, 9, MAX], [0, 5, MAX - 255, MAX - 254, MAX - 1, MAX, MAX], [0, MAX], [0, 0, 2, 2, 40, 700, 701],
                                    [0], [0, 1, 2, 1 << 29, 1 << 30]],
                          ids=lambda e: f"{len(e)}-borders-to-{e[-1]}")
 def test_borders_past_every_length(nrse_device, edges, T, causal):
