@@ -1134,8 +1134,9 @@ __global__ __launch_bounds__((256 * KvGeo<T, D>::ST)) __attribute__((amdgpu_wave
     }
   }
   if constexpr (ST > 1) {
-    // join: stream 0 leaves with dK, stream 1 with dV, each the sum in stream order
-    __syncthreads();
+    // join: stream 0 leaves with dK, stream 1 with dV, each the sum in stream order. (A slice without a pair comes
+    // here with its V copies still on their way, and the join's places lie over V's: they are waited for.)
+    wait_all_and_meet();
     float* const put = reinterpret_cast<float*>(dyn) + ((st == 0 ? 4 : 0) + w) * (D / 2) * 64 + lane;
     const float* const get = reinterpret_cast<const float*>(dyn) + ((st == 0 ? 0 : 4) + w) * (D / 2) * 64 + lane;
 #pragma unroll
