@@ -359,8 +359,9 @@ int nrse_attn_dropout_mask(uint16_t* drop_mask, int batch, int T, int H, float d
  * strides in elements, 16-byte multiples, row stride >= head_dim.
  *   s_ij = scale q_i.k_j + gate[h, i] * bias_vec[h, j - i + bias_len - 1]
  * bias_vec [hq, 2 * bias_len - 1] f32 (NULL: none) with bias_len >= every sequence's length; gate
- * [hq, rows] f32 (NULL: 1). A bias of -inf masks (with gate > 0); a row that is left nothing gives
- * zeros, lse = -inf and zero gradients. lse [hq, rows] f32 natural log (the forward may pass NULL).
+ * [hq, rows] f32 (NULL: 1). A bias of -inf masks (with gate > 0), and so does any large negative one
+ * where the row has another key; a row that is left nothing, or whose largest score under a bias is below
+ * -2^14 (the f32 lse could not tell its keys apart), gives zeros, lse = -inf and zero gradients. lse [hq, rows] f32 natural log (the forward may pass NULL).
  * cu_seqlens and seq_lens are device memory: what they hold is clamped to [0, rows], never trusted with
  * an address. A key row that holds NaN or infinity can reach the rows of its own sequence within
  * 128 rows before it under the causal mask (0 * NaN in a masked product), never another sequence.

@@ -33,6 +33,14 @@ constexpr float INF = __builtin_huge_valf();
 // Lazy rescaling: a row's probabilities are taken relative to a reference that only moves when a
 // score passes it by more than 2^8; f32 sums hold values up to 2^8 as well as values up to 1.
 constexpr float RESCALE_TAU = 8.f;
+// A score is rounded where it stands relative to the reference, so a reference far below it (a row whose first keys
+// are all masked by a large finite bias) would cost it bits of its own. A row has none, and is taken relative to
+// zero, until a score passes -2^6: the distance then rounds off less than a score of 2^6 does itself. A row that ends
+// without one is swept again relative to its largest score.
+constexpr float FLOOR = -64.f;
+// Under a bias, a row whose largest score is below -2^14 is taken to be left nothing: its keys are all masked by
+// finite values, and what they hide is less than the last f32 bit of an lse, by which the backward rebuilds P.
+constexpr float LEAST = -16384.f * LOG2E;
 
 NRSE_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -72,6 +80,14 @@ struct QGeo : Geo<T, D, tile_rows(D * (int)sizeof(T), (int)sizeof(T), ST)> {
   }
   static constexpr int Q_WAVES = B::RB > 256 ? 1 : 2;               // of dQ (three at 128-byte rows: no faster)
 };
+
+// LDS of dQ, and of the forward, which has a float for each row and stream behind it
+template <typename G>
+__host__ __device__ constexpr size_t lds_q(bool bias) {
+  return G::KV_LDS + (bias ? G::KV_LDS / (2 * G::BUF) * 8 * G::SEG * sizeof(float) : 0);
+}
+template <typename G>
+__host__ __device__ constexpr size_t lds_q_fwd(bool bias) { return lds_q<G>(bias) + 128 * sizeof(float); }
 
 // ---------------------------------------------------------------------------------- LDS tiles
 // Row r of a panel holds its 16-byte chunk c at position c ^ sw(r), sw(r) the three bits of (r / 2) % 8 in
@@ -351,6 +367,13 @@ NRSE_DEV void store4(T* p, float a, float b, float c, float d) {
   }
 }
 
+// The lane's number, formed where it is used: what is derived from it does not take registers through a loop.
+NRSE_DEV int lane_again() {
+  int zero = 0;
+  asm volatile("" : "+s"(zero));
+  return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+}
+
 NRSE_DEV void wait_all_and_meet() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -410,13 +433,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
   if constexpr (BIAS) bv_store<G::SEG>(bv0 + bst * 8 * G::SEG, bt, bv_load(vec, nd, e0));
   u32x4 qf[G::NS];
   const int qc = min(qi, len - 1);       // loads from a row that is there, zeroed after
-  const T* qrow = (const T*)p.q + (long long)(bl.seq0 + qc) * p.q_row + h * p.q_head;
+  auto load_q = [&]() {   // (and again before a second sweep: kept for that, registers ran out at head_dim 128)
+    const int ln = lane_again(), i = q0 + (ln & 31);
+    const T* qrow = (const T*)p.q + (long long)(bl.seq0 + min(i, len - 1)) * p.q_row + h * p.q_head;
 #pragma unroll
-  for (int s = 0; s < G::NS; ++s) {
-    qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qrow) + (2 * s + half) * 16);
-    if (qi >= len) qf[s] = u32x4{0, 0, 0, 0};
-  }
-  const float c1 = p.scale * LOG2E;
+    for (int s = 0; s < G::NS; ++s) {
+      qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qrow) + (2 * s + (ln >> 5)) * 16);
+      if (i >= len) qf[s] = u32x4{0, 0, 0, 0};
+    }
+  };
+  load_q();
+  const float c1 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(p.scale * LOG2E)));   // (a scalar register)
   float gl = LOG2E;
   if constexpr (BIAS) {
     if (p.gate) gl = p.gate[h * p.rows + bl.seq0 + qc] * LOG2E;
@@ -425,12 +452,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
   const float* const bcopy = bv0 + st * 8 * G::SEG + (u0 & 3) * G::SEG;
   const int uj = u0 - (u0 & 3), us = u0 & 3;
 
-  float mref = 0.f, thr = -INF, lsum = 0.f;
+  // thr: RESCALE_TAU once the row has a reference, its largest score (-inf: none) until then
+  float mref = 0.f, thr = -INF, lsum;
   f32x16 o[G::DT];
-#pragma unroll
-  for (int dt = 0; dt < G::DT; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
 
   auto tile = [&](const int it, auto masked_c) {
     constexpr bool MASKED = decltype(masked_c)::value;
@@ -507,13 +531,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
 #pragma unroll
         for (int r = 0; r < 16; r += 2) m4[(r >> 1) & 3] = fmaxf(fmaxf(m4[(r >> 1) & 3], v[t][r]), v[t][r + 1]);
       const float mx = xor32_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-      // thr: RESCALE_TAU once the row has a reference, -inf until then (a row whose bias is -inf
-      // so far has none)
       if (__builtin_amdgcn_ballot_w64(mx > thr)) {
-        const bool first = thr < 0.f;
-        const float sh = first ? (mx > -INF ? mx : 0.f) : fmaxf(mx, 0.f);
-        const float al = first ? 1.f : exp2_(-sh);
-        thr = mx > -INF ? RESCALE_TAU : thr;
+        const bool first = thr < 0.f, low = first && mx <= FLOOR;
+        const float sh = low ? 0.f : first ? mx : fmaxf(mx, 0.f);
+        const float al = exp2_(-sh);
+        thr = low ? fmaxf(thr, mx) : RESCALE_TAU;
         mref += sh;
         lsum *= al;
 #pragma unroll
@@ -543,16 +565,49 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
   };
   // tiles that every row of the workgroup sees whole, then those with a mask
   const int nfull = min(len, CAUSAL ? bl.row0 + 1 : len) / (KT * ST);
-  for (int it = 0; it < nfull; ++it) tile(it, std::false_type{});
-  for (int it = nfull; it < nit; ++it) tile(it, std::true_type{});
+  auto empty = [&]() {
+    lsum = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  };
+  empty();
+  for (bool again = false;; again = true) {
+    for (int it = 0; it < nfull; ++it) tile(it, std::false_type{});
+    for (int it = nfull; it < nit; ++it) tile(it, std::true_type{});
+    if (again) break;
+    // once more, where a row of the workgroup has no reference in any stream, but a score to take for one. (Every wave
+    // looks at all rows, so that all decide the same.)
+    float* const best = reinterpret_cast<float*>(dyn + lds_q_fwd<G>(BIAS)) - 128;   // [ST][BR]
+    const int ln = lane_again();
+    if (ln < 32) best[st * G::BR + sub * 32 + ln] = q0 + ln < len ? thr : 0.f;
+    __syncthreads();
+    float b = ST == 1 ? best[ln] : fmaxf(best[ln], best[64 + ln]);
+    bool redo = b < 0.f && b > (BIAS ? LEAST : -INF);
+    if constexpr (ST == 1) {
+      b = best[64 + ln];
+      redo |= b < 0.f && b > (BIAS ? LEAST : -INF);
+    }
+    if (!__builtin_amdgcn_ballot_w64(redo)) break;
+    if (thr < 0.f && thr > (BIAS ? LEAST : -INF)) {
+      mref = thr;
+      thr = RESCALE_TAU;
+    }
+    empty();
+    load_q();
+    issue(0);
+    if constexpr (BIAS) bv_store<G::SEG>(bv0 + bst * 8 * G::SEG, bt, bv_load(vec, nd, e0));
+  }
 
   float l = xor32_sum(lsum);
+  bool none = thr < 0.f;
   if constexpr (ST > 1) {
     // join: out = sum 2^(m_i - M) o_i over the streams, in stream order
     float* const js = reinterpret_cast<float*>(dyn);
     constexpr int PER = (D / 2 + 2) * 64;   // a wave's accumulators, maximum and sum
     float* const at = js + ((st - 1) * (4 / ST) + sub) * PER + lane;
-    const float mine = thr < 0.f ? -INF : mref;
+    const float mine = thr < 0.f ? -INF : mref;   // (-inf: relative to zero)
     __syncthreads();
     if (st > 0) {
 #pragma unroll
@@ -568,7 +623,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
     float M = mine;
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) M = fmaxf(M, from[i * (4 / ST) * PER + (D / 2) * 64]);
-    const float a0 = M > -INF ? exp2_(mine - M) : 0.f;
+    none = !(M > -INF);
+    // (a stream without a reference: relative to zero, and nothing in it where M is below FLOOR)
+    const float a0 = none ? 0.f : exp2_(fminf(mref - M, -FLOOR));
     l *= a0;
 #pragma unroll
     for (int dt = 0; dt < G::DT; ++dt)
@@ -577,26 +634,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) {
       const float* const x = from + i * (4 / ST) * PER;
-      const float a = M > -INF ? exp2_(x[(D / 2) * 64] - M) : 0.f;
+      const float mi = x[(D / 2) * 64];
+      const float a = none ? 0.f : exp2_(fminf((mi > -INF ? mi : 0.f) - M, -FLOOR));
       l = fmaf(a, x[(D / 2 + 1) * 64], l);
 #pragma unroll
       for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] = fmaf(a, x[(dt * 16 + r) * 64], o[dt][r]);
     }
-    mref = M > -INF ? M : 0.f;
+    mref = none ? 0.f : M;
   }
-  if (qi >= len) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row whose bias leaves nothing: zeros
-  T* const orow = (T*)p.out + (long long)(bl.seq0 + qi) * p.out_row + h * p.out_head + 4 * half;
+  const int ln = lane_again(), row = q0 + (ln & 31);
+  if (row >= len) return;
+  // a row whose bias leaves nothing: zeros; not one of NaN, whose sum is a NaN and no small number (seen by its bits: the
+  // compiler is told not to expect NaN)
+  none = none && __float_as_uint(l) < 0x40000000u;
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = none ? 0.f : o[dt][r] * inv;   // (a masked key's infinite value may be in its sums)
+  T* const orow = (T*)p.out + (long long)(bl.seq0 + row) * p.out_row + h * p.out_head + 4 * (ln >> 5);
 #pragma unroll
   for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
     for (int a = 0; a < 4; ++a)
-      store4<T>(orow + 32 * dt + 8 * a, o[dt][4 * a] * inv, o[dt][4 * a + 1] * inv, o[dt][4 * a + 2] * inv,
-                o[dt][4 * a + 3] * inv);
-  if (p.lse && half == 0)
-    p.lse[h * p.rows + bl.seq0 + qi] = l == 0.f ? -INF : (mref + __builtin_amdgcn_logf(l)) * LN2;
+      store4<T>(orow + 32 * dt + 8 * a, o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]);
+  if (p.lse && ln < 32)
+    p.lse[h * p.rows + bl.seq0 + row] = none ? -INF : (mref + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 // ---------------------------------------------------------------------------------- backward: dQ, dgate
@@ -1325,12 +1390,6 @@ __global__ __launch_bounds__(256) void rel_collect_kernel(const float* __restric
 }
 
 // ---------------------------------------------------------------------------------- launches
-template <typename T, int D, int ST>
-size_t lds_q(bool bias) {
-  using G = QGeo<T, D, ST>;
-  return G::KV_LDS + (bias ? ST * 8 * G::SEG * sizeof(float) : 0);
-}
-
 // Streams of the forward and dQ kernels: one where 128-row workgroups fill the chip (256 CUs take 512 at
 // once), two where they do not: under a causal mask, where half of them are short, it takes more. Measured,
 // forward / backward us in one stream and in two: full, 416 workgroups at head_dim 128 30 / 141 and 38 / 140, at 64
@@ -1377,7 +1436,7 @@ void launch_fwd(const nrse_attn_packed_fwd_params& p, hipStream_t st) {
   with_streams(q_streams(p.rows, p.nseq, p.hq, p.causal), [&](auto s) {
     constexpr int ST = decltype(s)::value;
     const long long n = grid_size(p.rows / (BQ / ST) + p.nseq, p.hkv, p.hq / p.hkv);
-    hipLaunchKernelGGL((fwd_kernel<T, D, BIAS, CAUSAL, ST>), dim3((unsigned)n), dim3(256), (lds_q<T, D, ST>(BIAS)), st, p);
+    hipLaunchKernelGGL((fwd_kernel<T, D, BIAS, CAUSAL, ST>), dim3((unsigned)n), dim3(256), (lds_q_fwd<QGeo<T, D, ST>>(BIAS)), st, p);
   });
 }
 
@@ -1393,7 +1452,7 @@ void launch_bwd(const nrse_attn_packed_bwd_params& p, hipStream_t st) {
   with_streams(q_streams(p.rows, p.nseq, p.hq, p.causal), [&](auto s) {
     constexpr int ST = decltype(s)::value;
     const long long n = grid_size(p.rows / (BQ / ST) + p.nseq, p.hkv, p.hq / p.hkv);
-    hipLaunchKernelGGL((bwd_q_kernel<T, D, BIAS, CAUSAL, ST>), dim3((unsigned)n), dim3(256), (lds_q<T, D, ST>(BIAS)), st, p);
+    hipLaunchKernelGGL((bwd_q_kernel<T, D, BIAS, CAUSAL, ST>), dim3((unsigned)n), dim3(256), (lds_q<QGeo<T, D, ST>>(BIAS)), st, p);
   });
   const int ns = kv_slices(p);
   float* const sums = ns > 1 ? p.part + slab_floats(p) : nullptr;
