@@ -356,7 +356,8 @@ int nrse_attn_dropout_mask(uint16_t* drop_mask, int batch, int T, int H, float d
  * batch); rows of no sequence are neither read into a result nor written. hq query heads over hkv
  * key heads (hq a multiple of hkv), head_dim 64 or 128, bf16 or f32 (exact f32 products), full or
  * causal (key <= query). Element (row, head, d) of x is at x + row * x_row + head * x_head + d:
- * strides in elements, 16-byte multiples, row stride >= head_dim.
+ * strides in elements, 16-byte multiples, row stride >= head_dim. What is written shares no memory with any other
+ * operand (views that interleave do not); such calls are refused.
  *   s_ij = scale q_i.k_j + gate[h, i] * bias_vec[h, j - i + bias_len - 1]
  * bias_vec [hq, 2 * bias_len - 1] f32 (NULL: none) with bias_len >= every sequence's length; gate
  * [hq, rows] f32 (NULL: 1). A bias of -inf masks (with gate > 0), and so does any large negative one

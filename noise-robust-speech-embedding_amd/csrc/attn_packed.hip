@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "overlap.h"
 
 namespace {
 
@@ -1513,13 +1514,24 @@ int check_common(const char* fn, const P* p) {
 }
 
 // what is written, and every other operand: an output's workgroups end while others still read
-int check_apart(const char* fn, std::initializer_list<const void*> outs, std::initializer_list<const void*> ins) {
+using nrse_overlap::Area;
+using nrse_overlap::flat;
+int check_apart(const char* fn, std::initializer_list<Area> outs, std::initializer_list<Area> ins) {
   for (auto o = outs.begin(); o != outs.end(); ++o) {
-    for (auto i = outs.begin(); i != o; ++i) NRSE_REQUIRE(*i != *o, "%s: two outputs at one address", fn);
-    for (const void* i : ins) NRSE_REQUIRE(i != *o, "%s: an output at an input's address", fn);
+    for (auto i = outs.begin(); i != o; ++i)
+      NRSE_REQUIRE(!o->at || !i->at || !meet(*o, *i), "%s: the outputs %s and %s share addresses", fn, i->name, o->name);
+    for (const Area& i : ins)
+      NRSE_REQUIRE(!o->at || !i.at || !meet(*o, i), "%s: the output %s shares addresses with %s", fn, o->name, i.name);
   }
   return NRSE_OK;
 }
+#define AREA(x, heads)                                                                                   \
+  Area {                                                                                                 \
+    #x, (uintptr_t)p->x, p->rows, p->x##_row * es, heads, p->x##_head * es, p->head_dim * es             \
+  }
+#define PER_ROW(x) flat(#x, p->x, 4LL * p->hq * p->rows)
+#define BIAS_SIZED(x) flat(#x, p->x, 4LL * p->hq * (2LL * p->bias_len - 1))
+#define LENGTHS flat("cu_seqlens", p->cu_seqlens, 4LL * p->nseq + 4), flat("seq_lens", p->seq_lens, 4LL * p->nseq)
 #define ROWS(fn, x) \
   if (const int rc = check_rows(fn, #x, p->x, p->x##_row, p->x##_head, p->dtype, p->head_dim, p->hq)) return rc
 #define ROWS_KV(fn, x) \
@@ -1538,7 +1550,10 @@ extern "C" int nrse_attn_packed_fwd(const nrse_attn_packed_fwd_params* p, void* 
   ROWS_KV(fn, k);
   ROWS_KV(fn, v);
   ROWS_OUT(fn, out, p->hq);
-  if (const int rc = check_apart(fn, {p->out}, {p->q, p->k, p->v})) return rc;
+  const long long es = p->dtype == NRSE_BF16 ? 2 : 4;
+  if (const int rc = check_apart(fn, {AREA(out, p->hq), PER_ROW(lse)},
+                                 {AREA(q, p->hq), AREA(k, p->hkv), AREA(v, p->hkv), PER_ROW(gate), BIAS_SIZED(bias_vec), LENGTHS}))
+    return rc;
   dispatch(*p, [&](auto t, auto d, auto b, auto c) {
     launch_fwd<decltype(t), decltype(d)::value, decltype(b)::value, decltype(c)::value>(*p, (hipStream_t)stream);
   });
@@ -1576,8 +1591,15 @@ extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* 
   ROWS_OUT(fn, dk, p->hkv);
   ROWS_OUT(fn, dv, p->hkv);
   NRSE_REQUIRE(p->lse && p->delta, "%s: lse and delta are needed", fn);
-  NRSE_REQUIRE(p->part || nrse_attn_packed_bwd_workspace(p) == 0, "%s: part, the workspace, is null", fn);
-  if (const int rc = check_apart(fn, {p->dq, p->dk, p->dv}, {p->q, p->k, p->v, p->out, p->dout})) return rc;
+  const long long floats = nrse_attn_packed_bwd_workspace(p), es = p->dtype == NRSE_BF16 ? 2 : 4;
+  NRSE_REQUIRE(p->part || floats == 0, "%s: part, the workspace, is null", fn);
+  NRSE_REQUIRE(((uintptr_t)p->part & 15) == 0, "%s: part, the workspace, is not 16-byte aligned", fn);
+  if (const int rc = check_apart(fn,
+                                 {AREA(dq, p->hq), AREA(dk, p->hkv), AREA(dv, p->hkv), PER_ROW(delta), PER_ROW(dgate),
+                                  BIAS_SIZED(dbias_vec), flat("part", p->part, 4 * floats)},
+                                 {AREA(q, p->hq), AREA(k, p->hkv), AREA(v, p->hkv), AREA(out, p->hq), AREA(dout, p->hq),
+                                  PER_ROW(lse), PER_ROW(gate), BIAS_SIZED(bias_vec), LENGTHS}))
+    return rc;
   dispatch(*p, [&](auto t, auto d, auto b, auto c) {
     launch_bwd<decltype(t), decltype(d)::value, decltype(b)::value, decltype(c)::value>(*p, st);
   });
@@ -1592,6 +1614,9 @@ extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* 
 extern "C" int nrse_rel_bias_expand(const float* E, const int* edges, int n, float* vec, int H, int T, int causal,
                                     void* stream) {
   NRSE_REQUIRE(E && edges && vec && n > 0 && H > 0 && T > 0 && T <= (1 << 29), "nrse_rel_bias_expand: bad args");
+  const Area in[] = {flat("E", E, 4LL * H * (causal ? n : 2LL * n)), flat("edges", edges, 4LL * n)},
+             out = flat("vec", vec, 4LL * H * (2LL * T - 1));
+  NRSE_REQUIRE(!meet(out, in[0]) && !meet(out, in[1]), "nrse_rel_bias_expand: vec shares addresses with E or edges");
   const long long blocks = (2LL * T - 1 + 255) / 256;
   // a head per workgroup row while that fills the chip, all of them in one loop for a long vector
   const unsigned rows = (unsigned)(blocks >= 1024 ? 1 : std::min(H, 65535));
@@ -1603,7 +1628,9 @@ extern "C" int nrse_rel_bias_expand(const float* E, const int* edges, int n, flo
 extern "C" int nrse_rel_bias_collect(const float* dvec, const int* edges, int n, float* dE, int H, int T, int causal,
                                      int accumulate, void* stream) {
   NRSE_REQUIRE(dvec && edges && dE && n > 0 && H > 0 && T > 0 && T <= (1 << 29), "nrse_rel_bias_collect: bad args");
-  const long long items = (long long)(causal ? n : 2 * n) * H;
+  const long long items = (causal ? n : 2LL * n) * H;
+  const Area in[] = {flat("dvec", dvec, 4LL * H * (2LL * T - 1)), flat("edges", edges, 4LL * n)}, out = flat("dE", dE, 4 * items);
+  NRSE_REQUIRE(!meet(out, in[0]) && !meet(out, in[1]), "nrse_rel_bias_collect: dE shares addresses with dvec or edges");
   NRSE_REQUIRE(items < (1LL << 24), "nrse_rel_bias_collect: %lld table entries", items);   // (2^32 threads)
   hipLaunchKernelGGL(rel_collect_kernel, dim3((unsigned)items), dim3(256), 0, (hipStream_t)stream, dvec, edges,
                      n, dE, H, T, causal, accumulate);
