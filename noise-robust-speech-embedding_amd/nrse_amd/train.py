@@ -63,14 +63,16 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     if not grads:
         return torch.tensor(0.0)
     # a dense gradient in another order of dimensions is the same values
-    grads = [g if g.is_contiguous() or not torch.ops.aten.is_non_overlapping_and_dense(g)
-             else g.as_strided((g.numel(),), (1,)) for g in grads]
+    flat = [g if g.is_contiguous() or not torch.ops.aten.is_non_overlapping_and_dense(g)
+            else g.as_strided((g.numel(),), (1,)) for g in grads]
     norm = torch.empty((), device=grads[0].device, dtype=torch.float32)
     if error_if_nonfinite:
-        K.grad_norm(grads, norm)
+        K.grad_norm(flat, norm)
         if not math.isfinite(float(norm)):
             raise RuntimeError(f"the gradients' norm is {float(norm)}: not clipped")
-    K.clip_grad_norm(grads, max_norm, norm)
+    K.clip_grad_norm(flat, max_norm, norm)
+    # the kernels write behind autograd's back: a graph that saved a gradient has to see that it changed
+    torch.autograd.graph.increment_version([g for g in grads if not g.is_inference()])
     return norm
 
 
