@@ -614,8 +614,8 @@ int nrse_sumsq(const float* x, long long n, double* out, double* part, void* str
  *   norm[0] = sqrt(sum x^2);  clip: x *= min(1, max_norm / (norm + 1e-6)), in place.
  * ptrs, numel, dtypes (NRSE_F32 or NRSE_BF16): HOST arrays of `count` contiguous device tensors, any
  * alignment their type allows; read before the call returns. part: nrse_grad_norm_workspace(...)
- * doubles. f64 sums in a fixed order. Clipping refuses tensors that overlap, and writes nothing where
- * the factor is 1; a NaN norm makes every value NaN. */
+ * doubles. f64 sums in a fixed order. norm and part lie in none of the tensors. Clipping refuses tensors
+ * that overlap, and writes nothing where the factor is 1; a NaN norm makes every value NaN. */
 long long nrse_grad_norm_workspace(const void* const* ptrs, const long long* numel, const int* dtypes, int count);
 int nrse_grad_norm(const void* const* ptrs, const long long* numel, const int* dtypes, int count, float* norm,
                    double* part, void* stream);

@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "common.h"
+#include "overlap.h"
 
 namespace {
 
@@ -186,6 +187,20 @@ int make_plan(const char* fn, const void* const* ptrs, const long long* numel, c
   return NRSE_OK;
 }
 
+// norm and part are written while tensors are read: in none of them, and apart
+int check_scratch(const char* fn, const void* const* ptrs, const long long* numel, const int* dtypes, int count, const Plan& pl,
+                  const float* norm, const double* part) {
+  using nrse_overlap::flat;
+  NRSE_REQUIRE(norm && part, "%s: norm or part is null", fn);
+  const auto n = flat("norm", norm, sizeof(float)), w = flat("part", part, (pl.chunks + 1) * (long long)sizeof(double));
+  NRSE_REQUIRE(!meet(n, w), "%s: norm and part overlap", fn);
+  for (int i = 0; i < count; ++i) {
+    const auto t = flat("", ptrs[i], numel[i] * es_of(dtypes[i]));
+    NRSE_REQUIRE(!meet(t, n) && !meet(t, w), "%s: tensor %d and norm or part overlap", fn, i);
+  }
+  return NRSE_OK;
+}
+
 template <typename F>
 void launches(const void* const* ptrs, const long long* numel, const int* dtypes, int count, const Plan& pl, bool backwards,
               F launch) {
@@ -238,7 +253,7 @@ extern "C" int nrse_grad_norm(const void* const* ptrs, const long long* numel, c
   const char* fn = "nrse_grad_norm";
   Plan pl;
   if (const int rc = make_plan(fn, ptrs, numel, dtypes, count, pl)) return rc;
-  NRSE_REQUIRE(norm && part, "%s: norm or part is null", fn);
+  if (const int rc = check_scratch(fn, ptrs, numel, dtypes, count, pl, norm, part)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   if (const int rc = run_norm(fn, ptrs, numel, dtypes, count, pl, part, st)) return rc;
   hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(1024), 0, st, part, (int)pl.chunks, norm, nullptr);
@@ -252,6 +267,7 @@ extern "C" int nrse_clip_grad_norm(const void* const* ptrs, const long long* num
   if (const int rc = make_plan(fn, ptrs, numel, dtypes, count, pl)) return rc;
   NRSE_REQUIRE(norm && part, "%s: norm or part is null", fn);
   NRSE_REQUIRE(max_norm >= 0.0, "%s: max_norm %g", fn, max_norm);
+  if (const int rc = check_scratch(fn, ptrs, numel, dtypes, count, pl, norm, part)) return rc;
   // two tensors that share an element would scale it twice, in any order
   try {
     std::vector<std::pair<uintptr_t, uintptr_t>> span;

@@ -83,3 +83,13 @@ def test_bias_tables():
         a.update(bad)
         assert L.nrse_rel_bias_collect(a["vec"], a["edges"], n, a["E"], H, T, 0, 0, None) < 0
         assert "share" in L.nrse_last_error().decode()
+
+
+@pytest.mark.parametrize("fn", ["nrse_grad_norm", "nrse_clip_grad_norm"])
+@pytest.mark.parametrize("norm,part", [(A + 16, A + FAR), (A + FAR, A - 8), (A + FAR, A + 4 * 100000 - 8), (A + FAR, A + FAR - 8)],
+                         ids=["norm-in-a-tensor", "part-before", "part-behind", "norm-in-part"])
+def test_gradient_norm_scratch_in_a_tensor(fn, norm, part):
+    L = _lib.lib()
+    a = ((ctypes.c_void_p * 2)(A + 2 * FAR, A), (ctypes.c_longlong * 2)(5, 100000), (ctypes.c_int * 2)(_lib.F32, _lib.F32), 2)
+    limit = () if fn == "nrse_grad_norm" else (1.0,)
+    assert getattr(L, fn)(*a, *limit, norm, part, None) < 0 and "overlap" in L.nrse_last_error().decode()
