@@ -49,7 +49,7 @@ NRSE_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // else 32. bf16 at head_dim 128: 32 rows let a third wave onto a SIMD (8192 causal rows, forward 280 -> 260 us;
 // 32 rows with two waves: 290). At head_dim 64, 32 rows and a fourth wave: no faster.
 constexpr int tile_rows(int row_bytes, int es, int ST) {
-  return row_bytes == 128 && ST <= 2 ? 64 : row_bytes == 256 && es == 4 && ST == 1 ? 64 : 32;
+  return row_bytes == 128 || (row_bytes == 256 && es == 4 && ST == 1) ? 64 : 32;
 }
 template <typename T, int D, int KT_>
 struct Geo {
@@ -64,14 +64,15 @@ struct Geo {
   static constexpr int SEG = 192;                       // bias entries of a workgroup's tile, KT + 127, in 64s
 };
 
-// The forward and dQ kernels in ST streams: the 4 waves are 4 / ST pieces of 32 rows times ST streams,
+// The forward and dQ kernels in ST streams, one or two: the 4 waves are 4 / ST pieces of 32 rows times ST streams,
 // and stream i takes every ST-th key tile, its running maximum, sum and output joined with the others' in
 // LDS at the end. A workgroup then has 128 / ST rows: more of them, each ST times shorter.
 template <typename T, int D, int ST>
 struct QGeo : Geo<T, D, tile_rows(D * (int)sizeof(T), (int)sizeof(T), ST)> {
   using B = Geo<T, D, tile_rows(D * (int)sizeof(T), (int)sizeof(T), ST)>;
   static constexpr int BR = 128 / ST;                               // rows of a workgroup
-  static constexpr int SEG = ST == 1 ? 192 : ST == 2 ? 128 : 64;    // >= KT + BR - 1, in 64s
+  static_assert(ST == 1 || ST == 2, "streams");
+  static constexpr int SEG = ST == 1 ? 192 : 128;                   // >= KT + BR - 1, in 64s
   static_assert(SEG >= B::KT + BR - 1 && SEG * ST <= 256, "a bias entry per thread");
   static constexpr int BUF = 2 * B::TILE;                           // K and V tile
   static constexpr int KV_LDS = ST * 2 * BUF;                       // [ST][2 buffers]
@@ -900,7 +901,8 @@ __host__ __device__ inline long long slab_row(int bias_len) { return ((bias_len 
 
 template <typename T, int D>
 struct KvGeo : Geo<T, D, (D * (int)sizeof(T) > 128 ? 32 : 64)> {
-  // bf16 at head_dim 128: the accumulators and K fill a wave's 256 registers, V's fragments stay in LDS
+  // bf16 at head_dim 128: the accumulators and K fill a wave's 256 registers, V's fragments stay in LDS. With a bias
+  // even so 42 registers of the compiler's report are spilled, and some of their reloads stand in the loop.
   static constexpr bool VLDS = sizeof(T) == 2 && D == 128;
   static constexpr int WAVES = sizeof(T) == 4 && D == 128 ? 1 : 2;   // per SIMD
   // Streams: where a workgroup's registers and LDS leave a SIMD two waves either way (256-byte rows), 8
