@@ -1467,7 +1467,9 @@ class ByolEngine:
     def embed(self, wav: torch.Tensor, which: str = "online", lengths=None) -> torch.Tensor:
         """The time-mean embedding [B, H] of wav [B, L]. lengths (samples, [B]: a sequence or an integer tensor): the
         utterances of a padded batch, each embedded as it would be alone; what the padding holds has no
-        part in it. An utterance shorter than one frame of the conv stack gives zeros."""
+        part in it, but is still computed through the conv stack and the linear layers. An utterance shorter than one
+        frame of the conv stack gives zeros. Host lengths outside [0, L] are refused; those of a device tensor, which
+        is not read back, are clamped."""
         self.sync_optimizer()
         flens = None if lengths is None else self.frame_lengths(lengths, wav)
         emb, _, _ = self.encoder_forward(self.weights(which), wav, train=False, flens=flens)
