@@ -1472,6 +1472,8 @@ class ByolEngine:
         is not read back, are clamped."""
         self.sync_optimizer()
         flens = None if lengths is None else self.frame_lengths(lengths, wav)
+        if flens is not None and self.arch.frames(wav.shape[1]) < 1:   # none of them has a frame
+            return torch.zeros(wav.shape[0], self.arch.hidden, device=self.dev, dtype=F32)
         emb, _, _ = self.encoder_forward(self.weights(which), wav, train=False, flens=flens)
         return emb
 

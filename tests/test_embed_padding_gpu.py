@@ -27,3 +27,12 @@ def test_device_lengths_are_clamped(nrse_device):
     over = torch.tensor([16000, 99999, -5, 400, 2 ** 40, 7777], device="cuda")
     assert torch.equal(eng.embed(wav, lengths=over), eng.embed(wav, lengths=[16000, 16000, 0, 400, 16000, 7777]))
     assert rel(eng.embed(wav, lengths=over)[[0]], alone(eng, wav)[[0]]) < 1e-4
+
+
+@pytest.mark.parametrize("L", [399, 300, 10, 9, 1])
+def test_a_batch_without_a_frame(nrse_device, L):
+    """Every utterance is shorter than one frame, and so is the batch: zeros, as for one such utterance among others."""
+    eng = engine(torch.float32)
+    wav = batch(0.0)[:, :L].contiguous()
+    emb = eng.embed(wav, lengths=[L, 0, 1, L, L, 0])
+    assert emb.shape == eng.embed(batch(0.0)).shape and emb.dtype == torch.float32 and (emb == 0).all()
