@@ -1506,7 +1506,7 @@ int check_common(const char* fn, const P* p) {
   NRSE_REQUIRE(p->rows >= 0 && p->rows < (1LL << 31) - 256 && p->nseq >= 0, "%s: rows %lld, sequences %d", fn, p->rows,
                p->nseq);
   NRSE_REQUIRE(p->nseq == 0 || p->cu_seqlens, "%s: cu_seqlens is null", fn);
-  NRSE_REQUIRE(!p->bias_vec || (p->bias_len > 0 && p->bias_len <= (1 << 29)), "%s: bias_len %d", fn, p->bias_len);
+  NRSE_REQUIRE(!p->bias_vec || (p->bias_len > 0 && p->bias_len < (1 << 29)), "%s: bias_len %d", fn, p->bias_len);
   NRSE_REQUIRE(p->bias_vec || !p->gate, "%s: a gate needs a bias", fn);
   // a grid has fewer than 2^32 threads: 512 of dK/dV's per 128 rows, 256 of dkv_kernel's per 32
   NRSE_REQUIRE(grid_size(p->rows / BQ + p->nseq, p->hkv, p->hq / p->hkv) < (1LL << 23) &&
@@ -1576,6 +1576,7 @@ extern "C" int nrse_attn_packed_bwd(const nrse_attn_packed_bwd_params* p, void* 
   if (const int rc = check_common(fn, p)) return rc;
   NRSE_REQUIRE(p->bias_vec || (!p->dbias_vec && !p->dgate), "%s: gradients of a bias that is not there", fn);
   NRSE_REQUIRE(p->gate || !p->dgate, "%s: dgate without a gate", fn);
+  NRSE_REQUIRE(!p->dbias_vec || p->hq < (1 << 16), "%s: the gradient of a bias of %d heads (65535 at most)", fn, p->hq);
   const hipStream_t st = (hipStream_t)stream;
   if (p->rows == 0 || p->nseq == 0) {
     if (p->dbias_vec && !p->accumulate) {

@@ -706,7 +706,8 @@ def attn_packed_fwd(q, k, v, cu_seqlens, out, lse=None, *, causal=False, scale=N
     cu_seqlens[s] .. cu_seqlens[s + 1] (int32, on the device), or, with seq_lens, the first seq_lens[s] of them (a
     padded batch); other rows of out and lse are left as they were. scale: default D^-1/2. lse: [hq, rows] f32 or
     None. bias_vec [hq, 2 T - 1] f32 with T >= every sequence (rel_bias_expand): + gate[h, i] * bias_vec[h, j - i +
-    T - 1] on the scores; gate [hq, rows] f32 or None (1)."""
+    T - 1] on the scores; gate [hq, rows] f32 or None (1). A bias of -inf, or a large negative one beside other keys,
+    masks; a row that is left nothing, or only scores below -2^14, gives zeros (lse -inf, no gradient)."""
     fn = "attn_packed_fwd"
     qs, ks, dt, dev, stream, lens, rest = _packed_args(fn, q, k, cu_seqlens, seq_lens, scale, gate, bias_vec)
     qp, qr, qh = _rows3(fn, "q", q, qs, dt, dev)

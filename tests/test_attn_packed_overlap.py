@@ -1,5 +1,5 @@
-"""Packed attention refuses outputs that share memory with any other operand, wholly or in part (CPU: refused on the host,
-before anything is launched)."""
+"""What packed attention and the gradient norm refuse on the host, before anything is launched (CPU): outputs that share
+memory with another operand, wholly or in part, and launches past their grid."""
 import ctypes
 import os
 
@@ -93,3 +93,17 @@ def test_gradient_norm_scratch_in_a_tensor(fn, norm, part):
     a = ((ctypes.c_void_p * 2)(A + 2 * FAR, A), (ctypes.c_longlong * 2)(5, 100000), (ctypes.c_int * 2)(_lib.F32, _lib.F32), 2)
     limit = () if fn == "nrse_grad_norm" else (1.0,)
     assert getattr(L, fn)(*a, *limit, norm, part, None) < 0 and "overlap" in L.nrse_last_error().decode()
+
+
+def test_launches_past_their_grid_are_refused_before_the_first():
+    """The bias gradient's launch has a head per grid row and a workgroup per 64 entries: refused where it could not
+    start, not after the other kernels have run."""
+    p = spread(bwd_params)
+    p.hq = p.hkv = 1 << 16
+    p.rows, p.nseq = 100, 1
+    for x in ("q", "k", "v", "out", "dout", "dq", "dk", "dv"):
+        setattr(p, x + "_row", 64 << 16)
+    assert "65535" in refusal(bwd_params, p)
+    p = spread(bwd_params)
+    p.bias_len = 1 << 29
+    assert "bias_len" in refusal(bwd_params, p)
