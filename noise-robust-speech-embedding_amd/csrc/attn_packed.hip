@@ -262,7 +262,9 @@ struct Dma {
 // ones fill the end. "Longest" by classes, each three quarters of the one before, of 64 sequences at a time, a
 // lane each: a place among them is a scan or two. (Against the batch's own order: 16 utterances, backward
 // 134 -> 113 us; 6 causal sequences, the longest last in that order, 162 -> 153. An exact order by 64 steps of
-// comparing: 64 sequences of 30 rows, forward 8 -> 20 us.) The grid is sized from what the host knows, rows / BR +
+// comparing: 64 sequences of 30 rows, forward 8 -> 20 us.) Every workgroup walks the sequences before its own, 64 at a
+// time, so with thousands of them the walk is most of the time: 8 heads of 64, sequences of 20 rows, 64 of them 7 us,
+// 1000 76, 4000 654. The grid is sized from what the host knows, rows / BR +
 // sequences, and what is left over ends at once.
 // Bounds are taken from cu_seqlens as they stand in device memory, clamped to the tensors.
 struct Block { int seq0, len, row0; bool any; };
@@ -384,11 +386,13 @@ NRSE_DEV void wait_all_and_meet() {
 
 // ---------------------------------------------------------------------------------- forward
 // Bound by the matrix units where there are rows enough (bf16): 8192 causal rows, 16 heads of 128 over 2,
-// 258-264 us = 1040-1065 TF (the matrix units busy 66 % of the time, no LDS conflicts, the rest exp and sums beside
-// them); long full sequences 1137 TF at 128, 950 at 64. Ragged batches are bound by each workgroup's own latency and
-// by the last ones to end: 4096 causal rows in 6 sequences, 16 heads of 128 over 4, 50 us; 16 utterances of 149 to
-// 599 rows, 16 heads of 64 with a bias, 32 us (matrix units 20 % busy, waves waiting 46 %). f32 is 16 times as
-// much matrix time a product: 1193 rows, 8 heads of 64, 32 us. A few single-token prompts: 6 us, the launch.
+// 256-278 us on several cards = 990-1075 TF (the matrix units busy 65 % of the time, no LDS conflicts, the rest exp and
+// sums beside them); long full sequences 1117 TF at 128, 941 at 64. Ragged batches are bound by each workgroup's own
+// latency and by the last ones to end: 4096 causal rows in 6 sequences, 16 heads of 128 over 4, 45 us; 16 utterances
+// of 149 to 599 rows, 16 heads of 64 with a bias, 31 us (matrix units 21 % busy, waves waiting 48 %). f32 is 16 times
+// as much matrix time a product: 1193 rows, 8 heads of 64, 31 us. A few single-token prompts: 6.3 us, the launch.
+// The second sweep, where it is needed, doubles a workgroup's time; asking whether it is, a barrier and two LDS reads,
+// takes up to 0.3 us of a call.
 template <typename T, int D, bool BIAS, bool CAUSAL, int ST>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::waves(BIAS), QGeo<T, D, ST>::waves(BIAS)))) void fwd_kernel(const nrse_attn_packed_fwd_params p) {
   using G = QGeo<T, D, ST>;
@@ -671,7 +675,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
 // delta is rowsum(dO O), from the stored output. The gradients of bias and gate are f32 outputs, and the
 // rounding of a bf16 O would be all their error (and a quarter of dK's): for what follows delta is summed again as
 // sum_j P dP from the f32 accumulators (EXACT), and dgate = sum P dP b - delta sum P b.
-// The forward's batches: 70 us (4096 causal rows), 51 us (utterances), 46 us (f32). It holds Q, dO, S and dP beside dQ, so
+// The forward's batches: 70-74 us (4096 causal rows), 51-53 us (utterances), 46 us (f32). It holds Q, dO, S and dP beside dQ, so
 // two waves per SIMD; what bounds it is the latency of one tile's chain of products and exponentials.
 template <typename T, int D, bool BIAS, bool CAUSAL, int ST>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, ST>::Q_WAVES, QGeo<T, D, ST>::Q_WAVES))) void bwd_q_kernel(const nrse_attn_packed_bwd_params p) {
@@ -884,9 +888,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QGeo<T, D, 
 // a thread each, in one order, into a ring; what the workgroup will not meet again leaves the ring for
 // this block's row of a slab in memory. rows of the slab are added by dbias_kernel: no atomics.
 //
-// Bound by latency at two waves per SIMD, and by the causal blocks' unequal lengths: the forward's batches take 89 us
-// (4096 causal rows; matrix units 31 % busy, waves waiting 46 %) + 14 us dkv_kernel, 69 us (utterances, with both the bias
-// and its gradient), 45 + 6 us (f32); long full sequences 800 TF for the whole backward at head_dim 128, 764 at 64.
+// Bound by latency at two waves per SIMD, and by the causal blocks' unequal lengths: the forward's batches take 89-94 us
+// (4096 causal rows; matrix units 29 % busy, waves waiting 47 %) + 14 us dkv_kernel, 69-73 us (utterances, with both the
+// bias and its gradient), 45 + 7 us (f32); long full sequences 676 TF for the whole backward at head_dim 128, 646 at 64.
 constexpr int RING = 256;   // more than the diagonals of an iteration
 template <int R>
 NRSE_DEV void diag_add(float v, float& lo, float& hi) {
@@ -1395,9 +1399,11 @@ __global__ __launch_bounds__(256) void rel_collect_kernel(const float* __restric
 // ---------------------------------------------------------------------------------- launches
 // Streams of the forward and dQ kernels: one where 128-row workgroups fill the chip (256 CUs take 512 at
 // once), two where they do not: under a causal mask, where half of them are short, it takes more. Measured,
-// forward / backward us in one stream and in two: full, 416 workgroups at head_dim 128 30 / 141 and 38 / 140, at 64
-// 17 / 50 and 17 / 49, 608 20 / 62 and 23 / 64, 288 13 / 44 and 13 / 43; causal, 672 at 128 77 / 262 and 68 / 257,
-// 720 at 64 43 / 181 and 44 / 178, 864 at 128 109 / 404 and 112 / 412.
+// forward / backward us in one stream and in two, 16 heads. One long sequence, full: 288 workgroups at head_dim 64
+// 43 / 147 and 41 / 141, 416 60 / 223 and 68 / 234, 416 at 128 96 / 423 and 112 / 436; causal: 672 at 128 150 / 498 and
+// 138 / 473, 720 at 64 100 / 330 and 95 / 328, 864 at 128 213 / 730 and 217 / 743. Five unequal ones, causal: 672 at 128
+// 62 / 191 and 54 / 178. Many short ones of one length are better off in one stream at any of these numbers (16 causal ones
+// of 208 rows, 672 at 128: 17 / 62 and 22 / 71), which the number of workgroups does not tell.
 int q_streams(long long rows, int nseq, int hq, int causal) {
   const long long n = (rows / BQ + nseq) * hq;
   return n >= (causal ? 700 : 400) ? 1 : 2;
@@ -1413,8 +1419,8 @@ size_t lds_kv(bool bias) {
 // causal sequence's first block, decides the time, and a batch with fewer blocks x key heads is split up
 // to 8 ways, each slice writing f32 sums that dkv_kernel adds. Not below 4 pairs a slice (of an average
 // sequence; 1 in f32, whose pairs take 8 times as long). Measured: causal f32 batch of 104 groups,
-// backward 139 us in 1 slice, 105 in 2, 89 in 4; causal bf16 of 152 groups 198 us in 2, 159 in 4, 175 in 7 (the sums'
-// traffic); 944 groups 141 us in 1, 173 in 2.
+// backward 144 us in 1 slice, 110 in 2, 94 in 4; causal bf16 of 152 groups 197 us in 2, 164 in 3, 155 in 4, 163 in 5,
+// 176 in 7 (the sums' traffic); 944 groups 94 us in 1, 162 in 2.
 int kv_slices(const nrse_attn_packed_bwd_params& p) {
   const long long groups = (p.rows / BQ + p.nseq) * p.hkv, G = p.hq / p.hkv;
   const bool f32 = p.dtype == NRSE_F32;
