@@ -416,8 +416,9 @@ long long nrse_attn_packed_bwd_workspace(const nrse_attn_packed_bwd_params* p);
 
 /* The bias vector of a learned table by buckets, for any length without a table per length: edges [n]
  * int32 ascending from 0 are the smallest distances of the n buckets of one side
- * (nrse_amd.hostside.bucket_edges); a border at or past T (up to 2^31 - 1) leaves its bucket empty. Two-sided (causal = 0): E [2n, H], keys at or behind the query take
- * rows 0 .. n-1, keys ahead n .. 2n-1. causal = 1: E [n, H], and a key ahead counts as distance 0.
+ * (nrse_amd.hostside.bucket_edges); a border at or past T (up to 2^31 - 1) leaves its bucket empty.
+ * Two-sided (causal = 0): E [2n, H], keys at or behind the query take rows 0 .. n-1, keys ahead n .. 2n-1.
+ * causal = 1: E [n, H], and a key ahead counts as distance 0.
  *   vec[h, d + T - 1] = E[bucket(d), h], |d| < T;   dE[b, h] (+)= sum of dvec[h, d + T - 1] over bucket b */
 int nrse_rel_bias_expand(const float* E, const int* edges, int n, float* vec, int H, int T, int causal, void* stream);
 int nrse_rel_bias_collect(const float* dvec, const int* edges, int n, float* dE, int H, int T, int causal,

@@ -16,3 +16,13 @@ def test_no_source_is_compiled_with_packed_f32():
     assert len(compiles) == sum(f.endswith(".hip") for f in os.listdir(CSRC))
     for line in compiles:
         assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in line, line
+
+
+def test_the_probes_say_the_same():
+    root = os.path.dirname(os.path.dirname(CSRC))
+    tools = os.path.join(root, "tools")
+    for name in sorted(os.listdir(tools)):
+        if name.endswith(".hip"):
+            with open(os.path.join(tools, name)) as f:
+                lines = [line for line in f if "hipcc" in line]
+            assert lines and all("-packed-fp32-ops" in line for line in lines), name

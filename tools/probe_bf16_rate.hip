@@ -2,7 +2,7 @@
 // accumulators) against v_mfma_f32_32x32x16_bf16 (4 independent 16-register accumulators), the
 // operands loop-invariant registers (no VALU in the loop), 2 workgroups of 4 waves per CU;
 // prints the whole-grid rate (dense FLOPs).
-// Build: hipcc --offload-arch=gfx950 -O3 tools/probe_bf16_rate.hip -o tools/probe_bf16_rate
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe_bf16_rate.hip -o tools/probe_bf16_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

@@ -2,7 +2,7 @@
 // one wave, exact small-integer data, per-lane block scales; the host checks each format against
 // the hypothesis "lane (g, i) holds row i's k = 32g .. 32g+31, value j at bits [w j, w j + w) of the
 // little-endian register string (w = 8 / 6 / 4), and its scale byte scales that 32-k block".
-// Build: hipcc --offload-arch=gfx950 -O2 tools/probe_mx.hip -o tools/probe_mx ; run on the GPU box.
+// Build: hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe_mx.hip -o tools/probe_mx
 #include <hip/hip_runtime.h>
 #include <cmath>
 #include <cstdio>

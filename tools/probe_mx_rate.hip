@@ -2,7 +2,7 @@
 // fp6 e2m3 = 2, fp4 e2m1 = 4) against v_mfma_f32_16x16x32_bf16: one workgroup of 4 waves per CU
 // (one per SIMD), each issuing a long chain over 8 independent accumulators; prints the cycles per
 // MFMA per SIMD from s_memtime and the whole-grid rate.
-// Build: hipcc --offload-arch=gfx950 -O3 tools/probe_mx_rate.hip -o tools/probe_mx_rate
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe_mx_rate.hip -o tools/probe_mx_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 
